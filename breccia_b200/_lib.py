@@ -22,6 +22,11 @@ ERR_NOT_RESIDENT = -8
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
+DTYPE_BF16 = 2
+
+KV8_CODES = {"e4m3": 1, "int8": 2}
+ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
 
 
 class BrcError(RuntimeError):
@@ -37,6 +42,12 @@ class Geometry(C.Structure):
     _fields_ = [("n_layers", C.c_uint32), ("n_kv_head", C.c_uint32), ("head_dim", C.c_uint32),
                 ("page_tokens", C.c_uint32), ("n_pages", C.c_uint32), ("device", C.c_int32),
                 ("half_page_bytes", C.c_uint64), ("total_bytes", C.c_uint64)]
+
+
+class RopeParams(C.Structure):
+    _fields_ = [("theta", C.c_double), ("factor", C.c_double), ("turns_low", C.c_double), ("turns_high", C.c_double),
+                ("mscale", C.c_double), ("n_rot", C.c_uint32), ("orig_ctx", C.c_uint32), ("scaling", C.c_int32),
+                ("reserved", C.c_int32)]
 
 
 _vp = C.c_void_p
@@ -131,6 +142,14 @@ SIGNATURES = {
     "brc_qk_prepare_append": [_vp, _u32, _vp, _u32, _u32, _vp, _vp, _vp, _vp, _f32, _vp, _u32, _u32, _vp, _u32, _vp, _u32, _u32,
                               _u32, _vp, _i32, _vp],
     "brc_paged_sparse_attn": [_vp, _u32, _vp, _i32, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _vp, _u32, _f32, _vp, _vp],
+    "brc_pool_create_kv8": [_i32, _u32, _u32, _u32, _u32, _u32, _i32, _vpp],
+    "brc_pool_kv8_code": [_vp, C.POINTER(C.c_int32)],
+    "brc_kv8_append": [_vp, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _u32, _vp, _u64, _vp, _u64, _i32, _vp, _u32, _i32, _f32, _vp],
+    "brc_kv8_read": [_vp, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _u32, _vp, _vp, _i32, _vp],
+    "brc_kv8_attn_workspace_bytes": [_vp, _u32, _u32, _u32, _u64p],
+    "brc_kv8_attn": [_vp, _u32, _vp, _i32, _u32, _vp, _u32, _vp, _u32, _vp, _vp, _u32, _u32, _u32, _f32, _vp, _i32, _vp, _u64, _vp],
+    "brc_rope_freqs": [C.POINTER(RopeParams), _u64p, C.POINTER(C.c_float)],
+    "brc_rope_apply": [_i32, _vp, _vp, _u32, _u64, _u64, _vp, _vp, _u32, _u64, _u64, _u32, _i32, _vp, _u32, _vp, _u32, _i32, _f32, _vp],
     "brc_timing_enable": [_vp, _i32],
     "brc_timing_read": [_vp, _i32, _u32p, C.POINTER(C.c_double)],
 }

@@ -17,6 +17,7 @@
 #define BRC_DEV_BAD_POS 2u     // position past the caller's bound
 #define BRC_DEV_WAIT_LIMIT 4u  // a bounded mbarrier wait gave up
 #define BRC_DEV_BAD_SHAPE 8u   // more work units than a kernel's table holds
+#define BRC_DEV_BAD_VALUE 16u  // a quantising write met an infinity or NaN
 
 // brc_pool::status_dev: 64 words of check state, then the decode kernels' per-unit arrival counters
 // (ticket words of the units, never cleared by the kernels: every launch adds a fixed amount per unit).
@@ -44,6 +45,10 @@ struct brc_pool {
     // V page bodies: binary16 like K, or q8_0 (blocks of 32 values: one f32 scale + 32 signed bytes, 36 B;
     // row = head_dim / 32 blocks; rows in the same order as the binary16 layout)
     bool v_q8 = false;
+    // 8-bit pages (brc_pool_create_kv8): 0 = not, else BRC_KV8_E4M3 / BRC_KV8_INT8.  A half page (K or V of one page
+    // of one layer) is then n_kv * page_tokens * head_dim codes followed by n_kv f32 scales, rounded up to 128 bytes.
+    uint32_t kv8 = 0;
+    alignas(64) CUtensorMap tm_kv8;   // (column, row of a page, page over all layers, K|V), box of brc_kv8_kvb heads' rows x 128 columns
     uint64_t v_layer_bytes = 0;     // V bytes of one layer: layer_bytes, or 9/16 of it for q8_0
     uint32_t *status_dev = nullptr; // device check word
     uint32_t *status_host = nullptr;  // pinned mirror
@@ -104,6 +109,15 @@ struct brc_pool {
                                       // is not "held by the caller": the tier neither offers nor demotes it)
     std::vector<uint32_t> free_list;  // LIFO
 };
+
+static inline uint32_t brc_kv8_kvb(const brc_pool *pool) { return pool->n_kv_head % 2u == 0u ? 2u : 1u; }   // kv heads of one unit
+
+// Entry points that read or write binary16 / q8_0 rows refuse a pool whose pages are 8-bit.
+#define BRC_REFUSE_KV8(pool, who, instead)                                                                              \
+    do {                                                                                                               \
+        if ((pool) && (pool)->kv8)                                                                                     \
+            return brc_fail(BRC_ERR_UNSUPPORTED, "%s: the pool's pages are 8-bit (brc_pool_create_kv8)%s", who, instead); \
+    } while (0)
 
 void brc_set_error(const char *fmt, ...) __attribute__((format(printf, 1, 2)));
 brc_status brc_fail(brc_status code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
@@ -177,6 +191,28 @@ struct brc_layers_args {
     uint64_t kv_layer_stride_bytes = 0;
     const brc_push_args *push = nullptr;
 };
+// Attention over 8-bit pages, as brc_kv8_attn and (for such pools) brc_paged_decode_attn call it (kv8_attn.cu).
+struct brc_kv8_attn_args {
+    uint32_t layer = 0;
+    const void *q = nullptr;
+    int32_t q_dtype = BRC_DTYPE_F16;
+    uint32_t n_head = 0;
+    const float *gate = nullptr;
+    uint32_t gate_head_stride = 0;
+    const uint32_t *block_tables = nullptr;
+    uint32_t table_stride = 0;
+    const uint32_t *seq_lens = nullptr;
+    const uint32_t *cu_q = nullptr;
+    uint32_t n_seqs = 0, max_seq_len = 0, max_q = 1;
+    float scale = 0.f;
+    void *out = nullptr;
+    int32_t out_dtype = BRC_DTYPE_F32;
+    void *workspace = nullptr;
+    uint64_t workspace_bytes = 0;
+};
+brc_status brc_kv8_attend(brc_pool *pool, const char *who, const brc_kv8_attn_args &a, void *stream);
+brc_status brc_kv8_workspace(const brc_pool *pool, uint32_t n_seqs, uint32_t n_head, uint32_t max_q, uint64_t *out_bytes);
+
 void brc_decode_calibrate(brc_pool *pool);
 brc_status brc_decode_layers(brc_pool *pool, const char *who, const brc_layers_args &args, void *stream);
 uint32_t brc_decode_kvb(const brc_pool *pool);   // kv heads that travel together in one unit (1 or 2)

@@ -1693,6 +1693,7 @@ brc_status note_decode_issued(brc_pool *pool, cudaStream_t st, bool capturing) {
 // Launches: one per (chunk of <= 2048 units per layer) x (group of layers whose partial slots fit the
 // workspace, at most BRC_DONE_BANKS) x (pass of GROUP_TILE query heads per kv head).
 brc_status brc_decode_layers(brc_pool *pool, const char *who, const brc_layers_args &a, void *stream) {
+    BRC_REFUSE_KV8(pool, who, "; brc_kv8_attn and brc_paged_decode_attn read them");
     if (brc_status rc = validate_decode(pool, who, a.layer0, a.n_layers, a.q, a.q_dtype, a.n_head, a.block_tables, a.table_stride,
                                         a.seq_lens, a.n_seqs, a.max_seq_len, a.out, a.workspace, a.workspace_bytes))
         return rc;
@@ -1875,7 +1876,7 @@ brc_status brc_decode_share_rates(const brc_pool *pool, float *rates, uint32_t c
 
 brc_status brc_decode_workspace_bytes(const brc_pool *pool, uint32_t n_seqs, uint32_t n_head, uint64_t *out_bytes) {
     if (!pool || !out_bytes) return brc_fail(BRC_ERR_INVALID, "brc_decode_workspace_bytes: NULL argument");
-    (void)n_head;
+    if (pool->kv8) return brc_kv8_workspace(pool, n_seqs, n_head, 1, out_bytes);
     *out_bytes = slots_for(pool, n_seqs) * slot_floats(pool) * sizeof(float);
     return BRC_OK;
 }
@@ -1885,6 +1886,27 @@ brc_status brc_paged_decode_attn(brc_pool *pool, uint32_t layer, const void *q_d
                                  uint32_t table_stride, const uint32_t *seq_lens_dev, uint32_t n_seqs,
                                  uint32_t max_seq_len, float scale, float *out_dev, void *workspace_dev,
                                  uint64_t workspace_bytes, void *stream) {
+    if (pool && pool->kv8) {
+        if (q_dtype != BRC_DTYPE_F32 && q_dtype != BRC_DTYPE_F16)
+            return brc_fail(BRC_ERR_INVALID, "brc_paged_decode_attn: q_dtype %d is neither f32 (0) nor f16 (1)", q_dtype);
+        brc_kv8_attn_args a;
+        a.layer = layer;
+        a.q = q_dev;
+        a.q_dtype = q_dtype;
+        a.n_head = n_head;
+        a.gate = gate_dev;
+        a.gate_head_stride = gate_head_stride;
+        a.block_tables = block_tables_dev;
+        a.table_stride = table_stride;
+        a.seq_lens = seq_lens_dev;
+        a.n_seqs = n_seqs;
+        a.max_seq_len = max_seq_len;
+        a.scale = scale;
+        a.out = out_dev;
+        a.workspace = workspace_dev;
+        a.workspace_bytes = workspace_bytes;
+        return brc_kv8_attend(pool, "brc_paged_decode_attn", a, stream);
+    }
     return brc_decode_layers(pool, "brc_paged_decode_attn",
                              one_layer(layer, q_dev, q_dtype, n_head, gate_dev, gate_head_stride, block_tables_dev, table_stride,
                                        seq_lens_dev, n_seqs, max_seq_len, scale, out_dev, workspace_dev, workspace_bytes),
@@ -1985,6 +2007,7 @@ brc_status brc_paged_decode_attn_static(brc_pool *pool, uint32_t layer, const vo
     if (!pool) return brc_fail(BRC_ERR_INVALID, "brc_paged_decode_attn_static: pool is NULL");
     if (pool->device < 0 || !pool->has_tma)
         return brc_fail(BRC_ERR_CUDA, "brc_paged_decode_attn_static: this pool holds bookkeeping only (no device memory)");
+    BRC_REFUSE_KV8(pool, "brc_paged_decode_attn_static", "; brc_kv8_attn and brc_paged_decode_attn read them");
     uint64_t need = 0;
     brc_decode_workspace_bytes(pool, n_seqs, n_head, &need);
     if (need > BRC_STATIC_WS_BYTES) {

@@ -219,6 +219,12 @@ brc_status brc_kv_append(brc_pool *pool, uint32_t layer, const uint32_t *block_t
                          const uint32_t *cu_tokens_dev, uint32_t total_tokens, uint32_t max_pos_end,
                          const void *k_src_dev, const void *v_src_dev, int32_t src_dtype, void *stream) {
     if (brc_status rc = need_device_pool(pool, "brc_kv_append")) return rc;
+    if (pool->kv8) {
+        if (src_dtype != BRC_DTYPE_F32 && src_dtype != BRC_DTYPE_F16)
+            return brc_fail(BRC_ERR_INVALID, "brc_kv_append: src_dtype %d is neither f32 (0) nor f16 (1)", src_dtype);
+        return brc_kv8_append(pool, layer, block_tables_dev, table_stride, pos0_dev, n_seqs, tokens_per_seq, cu_tokens_dev, total_tokens,
+                              max_pos_end, k_src_dev, 0, v_src_dev, 0, src_dtype, nullptr, 0, BRC_ROPE_HALF, 1.f, stream);
+    }
     if (pool->v_q8 && src_dtype != BRC_DTYPE_F32)
         return brc_fail(BRC_ERR_UNSUPPORTED, "brc_kv_append: a q8_0 V pool quantises from f32 sources only (src_dtype %d)", src_dtype);
     if (layer >= pool->n_layers)
@@ -273,6 +279,7 @@ brc_status brc_kv_append(brc_pool *pool, uint32_t layer, const uint32_t *block_t
 brc_status brc_page_gather(brc_pool *pool, uint32_t layer, const uint32_t *block_table_dev, uint32_t table_len,
                            uint32_t n_tokens, void *k_out_dev, void *v_out_dev, void *stream) {
     if (brc_status rc = need_device_pool(pool, "brc_page_gather")) return rc;
+    BRC_REFUSE_KV8(pool, "brc_page_gather", "; brc_kv8_read gives their values");
     if (layer >= pool->n_layers)
         return brc_fail(BRC_ERR_INVALID, "brc_page_gather: layer %u but the pool has %u", layer, pool->n_layers);
     if ((uint64_t)n_tokens > (uint64_t)table_len * pool->page_tokens)

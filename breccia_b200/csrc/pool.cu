@@ -174,8 +174,25 @@ static bool make_k_stage_map(CUtensorMap *tm, void *k_base, uint64_t rows, uint3
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// 4-D view of an 8-bit pool: (column, row of a half page, page of all layers, K|V).  One box brings 128 columns (the
+// swizzle span) of the K rows and of the V rows of `box_rows` / 16 kv heads of a page.
+static brc_status make_kv8_map(CUtensorMap *tm, const brc_pool *p, uint32_t box_rows) {
+    encode_tiled_fn enc = get_encode_tiled();
+    if (!enc) return brc_fail(BRC_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[4] = {p->head_dim, (cuuint64_t)p->n_kv_head * p->page_tokens, (cuuint64_t)p->n_layers * p->n_pages, 2u};
+    cuuint64_t strides[3] = {p->head_dim, p->half_page_bytes, p->layer_bytes * p->n_layers};
+    cuuint32_t box[4] = {128u, box_rows, 1u, 2u};
+    cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+    CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, p->k_base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return brc_fail(BRC_ERR_CUDA, "cuTensorMapEncodeTiled (8-bit view) failed with CUresult %d (%llu pages of %llu bytes)", (int)r,
+                        (unsigned long long)dims[2], (unsigned long long)p->half_page_bytes);
+    return BRC_OK;
+}
+
 static brc_status create_pool(int32_t device, uint32_t n_layers, uint32_t n_kv_head, uint32_t head_dim,
-                              uint32_t page_tokens, uint32_t n_pages, bool v_q8, brc_pool **out) {
+                              uint32_t page_tokens, uint32_t n_pages, bool v_q8, uint32_t kv8, brc_pool **out) {
     if (!out) return brc_fail(BRC_ERR_INVALID, "brc_pool_create: out is NULL");
     *out = nullptr;
     if (n_layers == 0 || n_kv_head == 0 || n_pages == 0)
@@ -206,6 +223,8 @@ static brc_status create_pool(int32_t device, uint32_t n_layers, uint32_t n_kv_h
     p->page_tokens = page_tokens;
     p->n_pages = n_pages;
     p->half_page_bytes = (uint64_t)n_kv_head * page_tokens * head_dim * 2u;
+    if (kv8) p->half_page_bytes = ((uint64_t)n_kv_head * (page_tokens * head_dim + sizeof(float)) + 127u) / 128u * 128u;
+    p->kv8 = kv8;
     p->layer_bytes = p->half_page_bytes * n_pages;
     const uint64_t bytes = p->layer_bytes * n_layers;
     p->v_q8 = v_q8;
@@ -230,15 +249,22 @@ static brc_status create_pool(int32_t device, uint32_t n_layers, uint32_t n_kv_h
         return rc;
     }
     cudaDeviceGetAttribute(&p->sm_count, cudaDevAttrMultiProcessorCount, device);
-    brc_status rc = make_map(&p->tm_k, p->k_base, rows, head_dim, page_tokens);
+    if (kv8) {   // its own view only: every entry point that uses the others refuses the pool
+        brc_status rc8 = make_kv8_map(&p->tm_kv8, p, brc_kv8_kvb(p) * page_tokens);
+        if (rc8 != BRC_OK) {
+            brc_pool_destroy(p);
+            return rc8;
+        }
+    }
+    brc_status rc = kv8 ? BRC_OK : make_map(&p->tm_k, p->k_base, rows, head_dim, page_tokens);
     // (a q8_0 V pool has no binary16 V rows to map: the kernels that use these views refuse it)
-    if (rc == BRC_OK && !v_q8) rc = make_map(&p->tm_v, p->v_base, rows, head_dim, page_tokens);
-    if (rc == BRC_OK && !v_q8) rc = make_kv_map(&p->tm_kv, p->k_base, bytes, rows, head_dim, page_tokens);
+    if (rc == BRC_OK && !v_q8 && !kv8) rc = make_map(&p->tm_v, p->v_base, rows, head_dim, page_tokens);
+    if (rc == BRC_OK && !v_q8 && !kv8) rc = make_kv_map(&p->tm_kv, p->k_base, bytes, rows, head_dim, page_tokens);
     // With an even number of kv heads, the rows of two neighbouring kv heads of a page are contiguous:
     // a box of 2 * page_tokens rows brings both (8 KiB per operation instead of 4 KiB).
-    if (rc == BRC_OK && !v_q8 && n_kv_head % 2u == 0u)
+    if (rc == BRC_OK && !v_q8 && !kv8 && n_kv_head % 2u == 0u)
         rc = make_kv_map(&p->tm_kv2, p->k_base, bytes, rows, head_dim, 2u * page_tokens);
-    if (rc == BRC_OK && !v_q8) {
+    if (rc == BRC_OK && !v_q8 && !kv8) {
         p->stage_maps = make_kv_stage_map(&p->tm_kv_stage, p->k_base, bytes, rows, head_dim, page_tokens) &&
                         (n_kv_head % 2u != 0u || make_kv_stage_map(&p->tm_kv2_stage, p->k_base, bytes, rows, head_dim, 2u * page_tokens));
     }
@@ -256,7 +282,7 @@ static brc_status create_pool(int32_t device, uint32_t n_layers, uint32_t n_kv_h
         return rc;
     }
     p->has_tma = true;
-    brc_decode_calibrate(p);   // per-SM streaming rates of this device (measured once per process; large pools only)
+    if (!kv8) brc_decode_calibrate(p);   // per-SM streaming rates of this device (measured once per process; large pools only)
     p->refcount.assign(n_pages, 0u);
     p->tree_refs.assign(n_pages, 0u);
     p->free_list.resize(n_pages);
@@ -269,16 +295,31 @@ extern "C" {
 
 brc_status brc_pool_create(int32_t device, uint32_t n_layers, uint32_t n_kv_head, uint32_t head_dim,
                            uint32_t page_tokens, uint32_t n_pages, brc_pool **out) {
-    return create_pool(device, n_layers, n_kv_head, head_dim, page_tokens, n_pages, false, out);
+    return create_pool(device, n_layers, n_kv_head, head_dim, page_tokens, n_pages, false, 0u, out);
 }
 
 brc_status brc_pool_create_q8v(int32_t device, uint32_t n_layers, uint32_t n_kv_head, uint32_t head_dim,
                                uint32_t page_tokens, uint32_t n_pages, brc_pool **out) {
-    return create_pool(device, n_layers, n_kv_head, head_dim, page_tokens, n_pages, true, out);
+    return create_pool(device, n_layers, n_kv_head, head_dim, page_tokens, n_pages, true, 0u, out);
+}
+
+brc_status brc_pool_create_kv8(int32_t device, uint32_t n_layers, uint32_t n_kv_head, uint32_t head_dim, uint32_t page_tokens,
+                               uint32_t n_pages, int32_t code, brc_pool **out) {
+    if (out) *out = nullptr;
+    if (code != BRC_KV8_E4M3 && code != BRC_KV8_INT8)
+        return brc_fail(BRC_ERR_INVALID, "brc_pool_create_kv8: code %d is neither e4m3 (1) nor int8 (2)", code);
+    return create_pool(device, n_layers, n_kv_head, head_dim, page_tokens, n_pages, false, (uint32_t)code, out);
+}
+
+brc_status brc_pool_kv8_code(const brc_pool *pool, int32_t *out_code) {
+    if (!pool || !out_code) return brc_fail(BRC_ERR_INVALID, "brc_pool_kv8_code: NULL argument");
+    *out_code = (int32_t)pool->kv8;
+    return BRC_OK;
 }
 
 brc_status brc_pool_v_layout(const brc_pool *pool, int32_t *out_layout) {
     if (!pool || !out_layout) return brc_fail(BRC_ERR_INVALID, "brc_pool_v_layout: NULL argument");
+    BRC_REFUSE_KV8(pool, "brc_pool_v_layout", "; brc_pool_kv8_code names their code");
     *out_layout = pool->v_q8 ? BRC_V_Q8_0 : BRC_V_F16;
     return BRC_OK;
 }
@@ -431,9 +472,10 @@ brc_status brc_pool_check(brc_pool *pool, void *stream) {
         return brc_fail(BRC_ERR_TIMEOUT, "a kernel gave up a bounded wait (check word 0x%x, detail %u, at %u of %u)", w, detail,
                         pool->status_host[2], pool->status_host[3]);
     return brc_fail(BRC_ERR_DEVICE_CHECK,
-                    "a kernel refused an index: check word 0x%x (%s%s%s), last offending value %u", w,
+                    "a kernel refused an index: check word 0x%x (%s%s%s%s), last offending value %u", w,
                     (w & BRC_DEV_BAD_PAGE) ? "page id >= n_pages " : "", (w & BRC_DEV_BAD_POS) ? "position past bound " : "",
-                    (w & BRC_DEV_BAD_SHAPE) ? "too many work units" : "", detail);
+                    (w & BRC_DEV_BAD_SHAPE) ? "too many work units" : "",
+                    (w & BRC_DEV_BAD_VALUE) ? "an infinity or NaN reached a quantising write" : "", detail);
 }
 
 brc_status brc_timing_enable(brc_pool *pool, int32_t on) {

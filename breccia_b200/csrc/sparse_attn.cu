@@ -638,6 +638,7 @@ brc_status brc_paged_sparse_attn(brc_pool *pool, uint32_t layer, const void *q_d
                                  const uint32_t *ids_dev, uint32_t max_ids, const uint32_t *counts_dev, uint32_t max_pos_end,
                                  float scale, float *out_dev, void *stream) {
     if (!pool) return brc_fail(BRC_ERR_INVALID, "brc_paged_sparse_attn: pool is NULL");
+    BRC_REFUSE_KV8(pool, "brc_paged_sparse_attn", "");
     if (pool->device < 0 || !pool->k_base)
         return brc_fail(BRC_ERR_CUDA, "brc_paged_sparse_attn: this pool holds bookkeeping only (no device memory)");
     if (layer >= pool->n_layers) return brc_fail(BRC_ERR_INVALID, "brc_paged_sparse_attn: layer %u but the pool has %u", layer, pool->n_layers);

@@ -430,7 +430,7 @@ struct ColdHeader {
     char magic[8];
     uint32_t n_layers, n_kv_head, head_dim, page_tokens;
     uint64_t slot_bytes;
-    uint32_t n_slots, reserved;
+    uint32_t n_slots, code;   // code: of 8-bit pages (their slots are of one size for e4m3 and int8), else 0
 };
 
 struct ColdEntry {
@@ -495,6 +495,7 @@ brc_status brc_cold_open(brc_tier *tier, const char *path, uint32_t n_slots, int
     want.head_dim = p->head_dim;
     want.page_tokens = p->page_tokens;
     want.slot_bytes = tier->slot_bytes;
+    want.code = p->kv8;
     brc_cold *c = new (std::nothrow) brc_cold();
     if (!c) return brc_fail(BRC_ERR_INVALID, "brc_cold_open: out of host memory");
     c->tier = tier;
@@ -522,14 +523,14 @@ brc_status brc_cold_open(brc_tier *tier, const char *path, uint32_t n_slots, int
             return brc_fail(BRC_ERR_INVALID, "brc_cold_open: %s is not a page store of this library", path);
         }
         if (h.n_layers != want.n_layers || h.n_kv_head != want.n_kv_head || h.head_dim != want.head_dim ||
-            h.page_tokens != want.page_tokens || h.slot_bytes != want.slot_bytes || h.n_slots == 0) {
+            h.page_tokens != want.page_tokens || h.slot_bytes != want.slot_bytes || h.code != want.code || h.n_slots == 0) {
             close(c->fd);
             delete c;
             return brc_fail(BRC_ERR_INVALID,
                             "brc_cold_open: %s holds pages of %u layers x %u kv heads x %u x %u cells (%llu bytes each); the pool's are "
-                            "%u x %u x %u x %u (%llu bytes)",
+                            "%u x %u x %u x %u (%llu bytes); 8-bit codes %u and %u",
                             path, h.n_layers, h.n_kv_head, h.head_dim, h.page_tokens, (unsigned long long)h.slot_bytes, want.n_layers,
-                            want.n_kv_head, want.head_dim, want.page_tokens, (unsigned long long)want.slot_bytes);
+                            want.n_kv_head, want.head_dim, want.page_tokens, (unsigned long long)want.slot_bytes, h.code, want.code);
         }
     }
     c->n_slots = h.n_slots;

@@ -37,13 +37,21 @@ def _u32_array(a) -> np.ndarray:
 class KvPool:
     """Paged f16 K/V pools of all layers on one GPU plus the page allocator (brc_pool).  v_q8: V page bodies
     as q8_0 blocks (the reference's VLayout::Q8_0, qsa/mod.rs:245-349): K stays binary16, append quantises
-    from f32, and every operator reads the blocks."""
+    from f32, and every operator reads the blocks.  kv8: K and V pages as 8-bit codes ("e4m3" or "int8") with one
+    power-of-two scale per page, kv head and side, for kv8_append / kv8_read / kv8_attend (and DecodeBatch.append /
+    attend)."""
 
     def __init__(self, device: int, n_layers: int, n_kv_head: int, head_dim: int, n_pages: int,
-                 page_tokens: int = PAGE_CELLS, bookkeeping_only: bool = False, v_q8: bool = False):
+                 page_tokens: int = PAGE_CELLS, bookkeeping_only: bool = False, v_q8: bool = False,
+                 kv8: str | None = None):
         self._h = C.c_void_p()
-        self.v_q8 = v_q8
-        if v_q8:
+        self.v_q8, self.kv8 = v_q8, kv8
+        if kv8 is not None:
+            if v_q8 or bookkeeping_only or kv8 not in _lib.KV8_CODES:
+                raise BrcError(_lib.ERR_INVALID, f"kv8={kv8!r}: \"e4m3\" or \"int8\", and neither v_q8 nor bookkeeping_only with it")
+            _lib.call("brc_pool_create_kv8", device, n_layers, n_kv_head, head_dim, page_tokens, n_pages, _lib.KV8_CODES[kv8],
+                      C.byref(self._h))
+        elif v_q8:
             _lib.call("brc_pool_create_q8v", device, n_layers, n_kv_head, head_dim, page_tokens, n_pages, C.byref(self._h))
         elif bookkeeping_only:
             _lib.call("brc_pool_create_bookkeeping", n_layers, n_kv_head, head_dim, page_tokens, n_pages,
@@ -55,6 +63,8 @@ class KvPool:
         self.n_layers, self.n_kv_head, self.head_dim = n_layers, n_kv_head, head_dim
         self.n_pages, self.page_tokens = n_pages, page_tokens
         self.half_page_bytes = n_kv_head * page_tokens * head_dim * 2
+        if kv8 is not None:   # one byte per value, then the heads' scales, to a multiple of 128 bytes
+            self.half_page_bytes = (n_kv_head * (page_tokens * head_dim + 4) + 127) // 128 * 128
 
     # -- lifetime
     @property
@@ -103,6 +113,8 @@ class KvPool:
         """Whole K (0) or V (1) pool of a layer as uint16 [n_pages, n_kv, page_tokens, head_dim]."""
         if which == 1 and self.v_q8:   # raw q8_0 rows: [n_pages * n_kv * page_tokens, head_dim / 32 * 36] bytes
             out = np.empty((self.n_pages * self.n_kv_head * self.page_tokens, self.head_dim // 32 * 36), np.uint8)
+        elif self.kv8 is not None:             # whole half pages: codes, then scales
+            out = np.empty((self.n_pages, self.half_page_bytes), np.uint8)
         else:
             out = np.empty((self.n_pages, self.n_kv_head, self.page_tokens, self.head_dim), np.uint16)
         _lib.call("brc_pool_read", self.handle, which, layer, 0, out.ctypes.data_as(C.c_void_p), out.nbytes,
@@ -113,6 +125,26 @@ class KvPool:
         data = np.ascontiguousarray(data)
         _lib.call("brc_pool_write", self.handle, which, layer, byte_offset, data.ctypes.data_as(C.c_void_p),
                   data.nbytes, _stream_ptr())
+
+    def kv8_view(self, which: int, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """The K (0) or V (1) pages of a layer of an 8-bit pool where they lie, as torch tensors: codes
+        [n_pages, n_kv, page_tokens, head_dim] (float8_e4m3fn or int8) and scales [n_pages, n_kv] f32.  Views of the
+        pool's own memory: valid until release(), written through at once."""
+        if self.kv8 is None:
+            raise BrcError(_lib.ERR_UNSUPPORTED, "kv8_view: the pool's pages are not 8-bit")
+        if which not in (0, 1):
+            raise BrcError(_lib.ERR_INVALID, f"kv8_view: which = {which} (0 = K, 1 = V)")
+        ptr = self.v_ptr(layer) if which else self.k_ptr(layer)
+        n, rows = self.n_pages * self.half_page_bytes, self.n_kv_head * self.page_tokens * self.head_dim
+
+        class Memory:
+            __cuda_array_interface__ = {"shape": (n,), "typestr": "|u1", "data": (ptr, False), "version": 3, "strides": None}
+
+        raw = torch.as_tensor(Memory(), device=f"cuda:{self.device}")
+        codes = raw.as_strided((self.n_pages, self.n_kv_head, self.page_tokens, self.head_dim),
+                               (self.half_page_bytes, self.page_tokens * self.head_dim, self.head_dim, 1))
+        scales = raw.view(torch.float32).as_strided((self.n_pages, self.n_kv_head), (self.half_page_bytes // 4, 1), rows // 4)
+        return codes.view(torch.float8_e4m3fn if self.kv8 == "e4m3" else torch.int8), scales
 
     # -- allocator
     def alloc(self, n: int) -> np.ndarray:
@@ -446,6 +478,156 @@ class IndexerState:
                   rows // rows_per_seq, rows_per_seq, n_blocks, IDX_DIM, IDX_BLOCK, 1.0 / math.sqrt(IDX_DIM), _ptr(scores),
                   _stream_ptr())
         return scores
+
+
+_DTYPES = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def _dtype(t: torch.dtype, who: str) -> int:
+    if t not in _DTYPES:
+        raise BrcError(_lib.ERR_INVALID, f"{who}: dtype {t} (float32, float16 or bfloat16)")
+    return _DTYPES[t]
+
+
+def _token_rows(t: torch.Tensor, heads: int, head_dim: int, who: str) -> int:
+    """Elements from one token's row [heads, head_dim] (or [heads * head_dim]) to the next; the row itself is contiguous."""
+    row = heads * head_dim
+    ok = (t.dim() == 2 and t.shape[1] == row and t.stride(1) == 1) or \
+         (t.dim() == 3 and t.shape[1:] == (heads, head_dim) and t.stride(2) == 1 and (heads == 1 or t.stride(1) == head_dim))
+    if not ok:
+        raise BrcError(_lib.ERR_INVALID, f"{who}: {tuple(t.shape)} with strides {t.stride()} is not rows of {heads} x {head_dim} values")
+    return t.stride(0) if t.shape[0] > 1 else row
+
+
+def _words(t: torch.Tensor, device: int, who: str, n: int | None = None) -> torch.Tensor:
+    """A contiguous array of 32-bit words on the pool's GPU (what positions, lengths, tables and prefixes are)."""
+    if t.dtype not in (torch.int32, torch.uint32) or not t.is_contiguous() or t.device.index != device or not t.is_cuda:
+        raise BrcError(_lib.ERR_INVALID, f"{who}: {t.dtype} {tuple(t.shape)} on {t.device}: contiguous 32-bit words on cuda:{device} wanted")
+    if n is not None and t.numel() != n:
+        raise BrcError(_lib.ERR_INVALID, f"{who}: {t.numel()} words, {n} wanted")
+    return t
+
+
+class Rope:
+    """Rotary positions without a cos / sin table: the first `n_rot` values of a head, in pairs (j, j + n_rot/2)
+    (layout "half") or (2j, 2j + 1) ("interleaved"), with frequencies theta^(-2j/n_rot) that `scaling` stretches for long
+    contexts: "linear", "ntk", "yarn", "bands" (include/breccia_kv.h, brc_rope_freqs; the reference has the half layout from a
+    host-built table, crates/breccia-kernels/src/qsa/mod.rs:1612-1614).  `turns_low` / `turns_high` bound yarn's and bands' transition,
+    in full turns over `orig_ctx` positions."""
+
+    def __init__(self, n_rot: int, theta: float = 10000.0, layout: str = "half", scaling: str = "none", factor: float = 1.0,
+                 orig_ctx: int = 0, turns_low: float = 1.0, turns_high: float | None = None, mscale: float = 0.0, device: int = 0):
+        if layout not in _lib.ROPE_LAYOUTS or scaling not in _lib.ROPE_SCALINGS:
+            raise BrcError(_lib.ERR_INVALID, f"Rope: layout {layout!r} of {list(_lib.ROPE_LAYOUTS)}, scaling {scaling!r} of {list(_lib.ROPE_SCALINGS)}")
+        if turns_high is None:
+            turns_high = 32.0 if scaling == "yarn" else 4.0
+        a = _lib.RopeParams(theta=theta, factor=factor, turns_low=turns_low, turns_high=turns_high, mscale=mscale, n_rot=n_rot,
+                            orig_ctx=orig_ctx, scaling=_lib.ROPE_SCALINGS[scaling])
+        self.turns_host = np.zeros(max(n_rot // 2, 1), np.uint64)   # fractions of a turn per position, times 2^64
+        f = C.c_float()
+        _lib.call("brc_rope_freqs", C.byref(a), self.turns_host.ctypes.data_as(C.POINTER(C.c_uint64)), C.byref(f))
+        self.factor, self.n_rot, self.layout, self.device = f.value, n_rot, _lib.ROPE_LAYOUTS[layout], device
+        self.turns = torch.from_numpy(self.turns_host.view(np.int64)).to(f"cuda:{device}") if torch.cuda.is_available() else None
+
+    def apply(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, q_out: torch.Tensor | None = None,
+              k_out: torch.Tensor | None = None, stream=None):
+        """q [tokens, n_head, head_dim], k [tokens, n_kv, head_dim] or None, positions [tokens] int32 -> (q_out, k_out), new
+        tensors unless given (q_out=q rotates in place).  Tokens may be strided (columns of one projection)."""
+        hd = q.shape[-1]
+        pair = []
+        for name, x, y in (("q", q, q_out), ("k", k, k_out)):
+            if x is None:
+                pair += [None, None, 0, 0, 0]
+                continue
+            if y is None:
+                y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            if x.dim() != 3 or x.shape[2] != hd or x.shape[0] != q.shape[0] or y.shape != x.shape or y.dtype != x.dtype or x.dtype != q.dtype:
+                raise BrcError(_lib.ERR_INVALID, f"Rope.apply: {name} {tuple(x.shape)} {x.dtype} -> {tuple(y.shape)} {y.dtype} beside q {tuple(q.shape)} {q.dtype}")
+            if not x.is_cuda or x.device.index != self.device or y.device != x.device:
+                raise BrcError(_lib.ERR_INVALID, f"Rope.apply: {name} on {x.device}, the frequencies on cuda:{self.device}")
+            pair += [x, y, x.shape[1], _token_rows(x, x.shape[1], hd, "Rope.apply"), _token_rows(y, x.shape[1], hd, "Rope.apply")]
+        _words(positions, self.device, "Rope.apply: positions", q.shape[0])
+        qi, qo, qh, qs, qos, ki, ko, kh, ks, kos = pair
+        _lib.call("brc_rope_apply", self.device, _ptr(qi), _ptr(qo), qh, qs, qos, _ptr(ki), _ptr(ko), kh, ks, kos, hd,
+                  _dtype(q.dtype, "Rope.apply"), _ptr(positions), q.shape[0], _ptr(self.turns), self.n_rot, self.layout, self.factor,
+                  _stream_ptr(stream))
+        return qo, ko
+
+
+def _kv8_spans(who: str, pool: KvPool, block_tables: torch.Tensor, pos0: torch.Tensor, cu_tokens, tokens_per_seq: int):
+    n_seqs = block_tables.shape[0]
+    _words(block_tables, pool.device, f"{who}: block_tables")
+    _words(pos0, pool.device, f"{who}: pos0", n_seqs)
+    if cu_tokens is not None:
+        _words(cu_tokens, pool.device, f"{who}: cu_tokens", n_seqs + 1)
+    return n_seqs, block_tables.shape[1]
+
+
+def kv8_append(pool: KvPool, layer: int, k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor, pos0: torch.Tensor,
+               max_pos_end: int, tokens_per_seq: int = 1, cu_tokens: torch.Tensor | None = None, rope: Rope | None = None,
+               stream=None) -> None:
+    """The quantising write into an 8-bit pool (brc_kv8_append): k / v [total_tokens, n_kv, hd] (tokens may be strided) at cells
+    pos0[s] .. of each sequence, tokens_per_seq each or ragged by cu_tokens [n_seqs + 1] int32; `rope` rotates K on the way."""
+    n_seqs, stride = _kv8_spans("kv8_append", pool, block_tables, pos0, cu_tokens, tokens_per_seq)
+    if k.dtype != v.dtype or k.shape[0] != v.shape[0] or not k.is_cuda or k.device.index != pool.device or v.device != k.device:
+        raise BrcError(_lib.ERR_INVALID, f"kv8_append: k {tuple(k.shape)} {k.dtype} {k.device}, v {tuple(v.shape)} {v.dtype} {v.device}")
+    if rope is not None and rope.device != pool.device:
+        raise BrcError(_lib.ERR_INVALID, f"kv8_append: the frequencies lie on cuda:{rope.device}, the pool on cuda:{pool.device}")
+    _lib.call("brc_kv8_append", pool.handle, layer, _ptr(block_tables), stride, _ptr(pos0), n_seqs, tokens_per_seq, _ptr(cu_tokens),
+              k.shape[0], max_pos_end, _ptr(k), _token_rows(k, pool.n_kv_head, pool.head_dim, "kv8_append"), _ptr(v),
+              _token_rows(v, pool.n_kv_head, pool.head_dim, "kv8_append"), _dtype(k.dtype, "kv8_append"),
+              _ptr(rope.turns) if rope else None, rope.n_rot if rope else 0, rope.layout if rope else 0, rope.factor if rope else 1.0,
+              _stream_ptr(stream))
+
+
+def kv8_read(pool: KvPool, layer: int, block_tables: torch.Tensor, pos0: torch.Tensor, max_pos_end: int, tokens_per_seq: int = 1,
+             cu_tokens: torch.Tensor | None = None, total_tokens: int | None = None, dtype: torch.dtype = torch.float16,
+             stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cells pos0[s] .. of each sequence of an 8-bit pool as values (brc_kv8_read) -> K, V [total_tokens, n_kv, hd]."""
+    n_seqs, stride = _kv8_spans("kv8_read", pool, block_tables, pos0, cu_tokens, tokens_per_seq)
+    if total_tokens is None:
+        if cu_tokens is not None:
+            raise BrcError(_lib.ERR_INVALID, "kv8_read: total_tokens is needed beside cu_tokens")
+        total_tokens = n_seqs * tokens_per_seq
+    out = torch.empty((2, total_tokens, pool.n_kv_head, pool.head_dim), dtype=dtype, device=block_tables.device)
+    k, v = out.unbind(0)
+    _lib.call("brc_kv8_read", pool.handle, layer, _ptr(block_tables), stride, _ptr(pos0), n_seqs, tokens_per_seq, _ptr(cu_tokens),
+              total_tokens, max_pos_end, _ptr(k), _ptr(v), _dtype(dtype, "kv8_read"), _stream_ptr(stream))
+    return k, v
+
+
+def kv8_workspace(pool: KvPool, n_seqs: int, n_head: int, max_q: int = 1) -> torch.Tensor:
+    """The scratch kv8_attend needs for calls of at most these sizes."""
+    need = C.c_uint64()
+    _lib.call("brc_kv8_attn_workspace_bytes", pool.handle, n_seqs, n_head, max_q, C.byref(need))
+    return torch.empty(need.value, dtype=torch.uint8, device=f"cuda:{pool.device}")
+
+
+def kv8_attend(pool: KvPool, layer: int, q: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, max_seq_len: int,
+               workspace: torch.Tensor, max_q: int = 1, cu_q: torch.Tensor | None = None, scale: float | None = None,
+               out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None, gate: torch.Tensor | None = None,
+               gate_head_stride: int = 0, stream=None) -> torch.Tensor:
+    """Attention over an 8-bit pool for the last T tokens of each sequence (brc_kv8_attn): q [tokens, n_head, hd], T = max_q, or
+    ragged by cu_q [n_seqs + 1] int32 with T <= max_q; token i of T sees seq_lens[s] - (T - 1 - i) cells.  `workspace` from
+    kv8_workspace; calls that may run at the same time need one each."""
+    n_seqs = block_tables.shape[0]
+    _words(block_tables, pool.device, "kv8_attend: block_tables")
+    _words(seq_lens, pool.device, "kv8_attend: seq_lens", n_seqs)
+    if cu_q is not None:
+        _words(cu_q, pool.device, "kv8_attend: cu_q", n_seqs + 1)
+    elif q.shape[0] != n_seqs * max_q:
+        raise BrcError(_lib.ERR_INVALID, f"kv8_attend: {q.shape[0]} rows of q for {n_seqs} sequences of {max_q} tokens")
+    if q.dim() != 3 or q.shape[2] != pool.head_dim or not q.is_contiguous() or not q.is_cuda or q.device.index != pool.device:
+        raise BrcError(_lib.ERR_INVALID, f"kv8_attend: q {tuple(q.shape)} on {q.device}: contiguous [tokens, n_head, {pool.head_dim}] wanted")
+    if out is None:
+        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
+    elif out.shape != q.shape or not out.is_contiguous() or out.device != q.device:
+        raise BrcError(_lib.ERR_INVALID, f"kv8_attend: out {tuple(out.shape)} on {out.device} beside q {tuple(q.shape)}")
+    _lib.call("brc_kv8_attn", pool.handle, layer, _ptr(q), _dtype(q.dtype, "kv8_attend"), q.shape[1], _ptr(gate), gate_head_stride,
+              _ptr(block_tables), block_tables.shape[1], _ptr(seq_lens), _ptr(cu_q), n_seqs, max_q, max_seq_len,
+              1.0 / math.sqrt(pool.head_dim) if scale is None else scale, _ptr(out), _dtype(out.dtype, "kv8_attend"), _ptr(workspace),
+              workspace.numel() * workspace.element_size(), _stream_ptr(stream))
+    return out
 
 
 def decode_partial_bytes(n_seqs: int, n_head: int, head_dim: int) -> int:

@@ -57,6 +57,7 @@ typedef int32_t brc_status;
 /* dtype tags for query / source tensors */
 #define BRC_DTYPE_F32 0
 #define BRC_DTYPE_F16 1
+#define BRC_DTYPE_BF16 2 /* the rotary and 8-bit-page entry points only */
 
 typedef struct brc_pool brc_pool;
 typedef struct brc_radix brc_radix;
@@ -115,6 +116,25 @@ BRC_API brc_status brc_pool_create(int32_t device, uint32_t n_layers, uint32_t n
 BRC_API brc_status brc_pool_create_q8v(int32_t device, uint32_t n_layers, uint32_t n_kv_head, uint32_t head_dim,
                                        uint32_t page_tokens, uint32_t n_pages, brc_pool **out);
 BRC_API brc_status brc_pool_v_layout(const brc_pool *pool, int32_t *out_layout);
+/* A pool whose pages are 8-bit, K and V alike (no counterpart in the reference).
+ * A half page (K or V of one page of one layer) is
+ *   codes  [n_kv_head][16 cells][head_dim], one byte each, then
+ *   scales [n_kv_head] f32,
+ * rounded up to 128 bytes; a value is code * scale.  ONE scale per page, kv head
+ * and side, always a power of two 2^e with -120 <= e <= 120.  Codes are e4m3
+ * (finite ones only: |code| <= 448) or signed bytes (|code| <= 127).  1040 bytes
+ * of K and V per cell instead of 2048 at 2 kv heads of 256.  Built for such a pool:
+ * brc_kv8_append / brc_kv8_read / brc_kv8_attn below; brc_kv_append (f32 or f16
+ * sources) and brc_paged_decode_attn, which call them; brc_page_copy,
+ * brc_seq_fork, brc_tier_*, brc_cold_* and brc_pool_read / _write / _zero (whole
+ * pages, scales included); the allocator and the prefix tree.  Every other entry
+ * point that reads or writes pages refuses it with BRC_ERR_UNSUPPORTED. */
+#define BRC_KV8_E4M3 1
+#define BRC_KV8_INT8 2
+BRC_API brc_status brc_pool_create_kv8(int32_t device, uint32_t n_layers, uint32_t n_kv_head, uint32_t head_dim,
+                                       uint32_t page_tokens, uint32_t n_pages, int32_t code, brc_pool **out);
+/* *out_code: BRC_KV8_E4M3, BRC_KV8_INT8, or 0 for a pool that is not 8-bit. */
+BRC_API brc_status brc_pool_kv8_code(const brc_pool *pool, int32_t *out_code);
 /* A pool without device memory: page ids, refcounts and (later) prefix-tree and
  * tier bookkeeping only.  Every entry point that would touch the GPU refuses it
  * with BRC_ERR_CUDA.  Exists so schedulers and tests can exercise the host-side
@@ -308,6 +328,111 @@ BRC_API brc_status brc_paged_decode_attn_static(brc_pool *pool, uint32_t layer, 
                                                 const uint32_t *block_tables_dev, uint32_t table_stride,
                                                 const uint32_t *seq_lens_dev, uint32_t n_seqs, uint32_t max_seq_len,
                                                 float scale, float *out_dev, void *stream);
+
+/* ---------------------------------------------------------------- 8-bit pages (no counterpart in the reference)
+ * brc_kv8_append: the quantising write, with brc_kv_append's arguments: sequence
+ * s puts its tokens at cells pos0_dev[s] .. .  Sources are f32, f16 or bf16 rows
+ * of n_kv_head * head_dim values, `*_token_stride` ELEMENTS apart (0: packed; a
+ * stride lets K and V be columns of one projection).  Per page, kv head and side:
+ *   need = least e with max|x| <= 448 * 2^e (e4m3) or 127 * 2^e (int8) over the
+ *          finite values this call writes there, clamped to -120 .. 120
+ *   e'   = need when the call writes the page's cell 0, else max(e, need) with
+ *          the page's present e
+ *   new cells:  code = x / 2^e' rounded to nearest, ties to even
+ *   kept cells (in front of the first one written): rounded again to 2^e' when
+ *          the scale grew.
+ * Infinities saturate, NaN is stored as 0, and either is reported through
+ * brc_pool_check.  A sequence ends where its last append ended: cells of its last
+ * page behind that are undefined (rolling back means appending at a smaller
+ * pos0; the page's scale then stays what it had grown to).  Two sequences of one
+ * call must not write one page.
+ *   rope_turns_dev  non-NULL: K is rotated on the way, cell c at position c, as
+ *     brc_rope_apply would with the same n_rot, rope_layout and rope_factor.
+ * brc_kv8_read: cells pos0_dev[s] .. of each sequence as values, packed
+ * [total_tokens][n_kv_head][head_dim] f32, f16 or bf16 (rounded once; f32 and,
+ * for int8 codes, bf16 are exact unless out of range).  Outputs 16-byte aligned. */
+#define BRC_ROPE_HALF 0        /* pairs (j, j + n_rot / 2) */
+#define BRC_ROPE_INTERLEAVED 1 /* pairs (2 j, 2 j + 1)     */
+BRC_API brc_status brc_kv8_append(brc_pool *pool, uint32_t layer, const uint32_t *block_tables_dev, uint32_t table_stride,
+                                  const uint32_t *pos0_dev, uint32_t n_seqs, uint32_t tokens_per_seq,
+                                  const uint32_t *cu_tokens_dev, uint32_t total_tokens, uint32_t max_pos_end,
+                                  const void *k_src_dev, uint64_t k_token_stride, const void *v_src_dev,
+                                  uint64_t v_token_stride, int32_t src_dtype, const uint64_t *rope_turns_dev,
+                                  uint32_t n_rot, int32_t rope_layout, float rope_factor, void *stream);
+BRC_API brc_status brc_kv8_read(brc_pool *pool, uint32_t layer, const uint32_t *block_tables_dev, uint32_t table_stride,
+                                const uint32_t *pos0_dev, uint32_t n_seqs, uint32_t tokens_per_seq,
+                                const uint32_t *cu_tokens_dev, uint32_t total_tokens, uint32_t max_pos_end,
+                                void *k_out_dev, void *v_out_dev, int32_t out_dtype, void *stream);
+/* Attention over 8-bit pages for one or several tokens per sequence (drafted
+ * tokens, the end of a prompt): sequence s has T(s) rows of q, the last T(s) of
+ * its seq_lens_dev[s] cells - T uniform (`max_q`, cu_q_dev == NULL) or ragged
+ * (cu_q_dev[n_seqs + 1] exclusive prefix; max_q bounds T) - and
+ *   out[i, h] = sigmoid(gate[i, h]) * softmax_c(scale * q[i, h] . k_c) . v_c
+ * over the cells c < seq_lens[s] - (T - 1 - i), kv head = h * n_kv_head / n_head.
+ * A row that sees no cell yields zeros.  Cells at or past seq_lens[s] never
+ * reach a result.  q and out are packed [tokens][n_head][head_dim], f32, f16 or
+ * bf16 each; gate as in brc_paged_decode_attn.  The dot products and the
+ * softmax are carried in f32 over exact products of the codes; the
+ * probabilities are rounded to binary16 when both q and out are 16-bit and kept
+ * as two binary16 parts (22 bits) otherwise.  A row with an infinity or NaN in q yields NaN.
+ * Up to 32 rows (T x heads per kv head) share one stream of the cache; more are
+ * taken in passes of 32, each streaming it again: made for decode and drafts,
+ * not for long prompts.
+ * workspace_dev: brc_kv8_attn_workspace_bytes() for these n_seqs, n_head, max_q;
+ * 16-byte aligned, contents undefined before and after.  Nothing outside it is
+ * shared between calls: calls with workspaces of their own may run at the same
+ * time, on one pool too, and captured ones may be replayed side by side. */
+BRC_API brc_status brc_kv8_attn_workspace_bytes(const brc_pool *pool, uint32_t n_seqs, uint32_t n_head, uint32_t max_q,
+                                                uint64_t *out_bytes);
+BRC_API brc_status brc_kv8_attn(brc_pool *pool, uint32_t layer, const void *q_dev, int32_t q_dtype, uint32_t n_head,
+                                const float *gate_dev, uint32_t gate_head_stride, const uint32_t *block_tables_dev,
+                                uint32_t table_stride, const uint32_t *seq_lens_dev, const uint32_t *cu_q_dev,
+                                uint32_t n_seqs, uint32_t max_q, uint32_t max_seq_len, float scale, void *out_dev,
+                                int32_t out_dtype, void *workspace_dev, uint64_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------- rotary positions
+ * The rotation of Qsa::rope_q / rope_k (crates/breccia-kernels/src/qsa/mod.rs:
+ * 1612-1614, shaders/ops_rope.comp:62-95) without its cos / sin table, in both
+ * pair layouts and with frequencies scaled for long contexts (the reference has
+ * the half layout, from a host-built table).  brc_qk_prepare_append keeps the
+ * table form, fused with the norms.
+ *
+ * brc_rope_freqs (host): the frequencies f_j = theta^(-2j / n_rot) of the
+ * n_rot / 2 pairs, scaled, as fractions of a turn per position times 2^64, and
+ * the factor on the rotated values.
+ *   LINEAR  f / factor
+ *   NTK     theta * factor^(n_rot / (n_rot - 2)) in place of theta
+ *   YARN    f between f and f / factor by the pair's index (full turns over
+ *           orig_ctx from turns_high down to turns_low); factor 0.1 ln(factor) + 1
+ *   BANDS   f between f and f / factor by the pair's number of turns over orig_ctx
+ * mscale > 0 replaces the scaling's own factor.
+ * brc_rope_apply: rotates q and / or k rows [n_tokens][heads][head_dim] (NULL: the
+ * other alone), f32, f16 or bf16, computed in f32; dims at and past n_rot are
+ * copied.  Token strides in elements, 0: packed.  An output may be its input, the
+ * same rows; otherwise the two must not overlap. */
+#define BRC_ROPE_NONE 0
+#define BRC_ROPE_LINEAR 1
+#define BRC_ROPE_NTK 2
+#define BRC_ROPE_YARN 3
+#define BRC_ROPE_BANDS 4
+typedef struct brc_rope_params {
+    double theta;
+    double factor;    /* >= 1; ignored by BRC_ROPE_NONE               */
+    double turns_low; /* YARN and BANDS: at or below, f / factor      */
+    double turns_high;/* YARN and BANDS: at or above, f               */
+    double mscale;    /* 0: the scaling's own                         */
+    uint32_t n_rot;   /* even, 2 .. 256                               */
+    uint32_t orig_ctx;/* YARN and BANDS: positions the model was trained on */
+    int32_t scaling;
+    int32_t reserved;
+} brc_rope_params;
+BRC_API brc_status brc_rope_freqs(const brc_rope_params *params, uint64_t *out_turns, float *out_factor);
+BRC_API brc_status brc_rope_apply(int32_t device, const void *q_dev, void *q_out_dev, uint32_t n_head,
+                                  uint64_t q_token_stride, uint64_t q_out_token_stride, const void *k_dev,
+                                  void *k_out_dev, uint32_t n_kv_head, uint64_t k_token_stride,
+                                  uint64_t k_out_token_stride, uint32_t head_dim, int32_t dtype,
+                                  const uint32_t *positions_dev, uint32_t n_tokens, const uint64_t *turns_dev,
+                                  uint32_t n_rot, int32_t layout, float factor, void *stream);
 
 /* ---------------------------------------------------------------- split-KV across GPUs
  * One long sequence whose cells are split into contiguous, page-aligned ranges

@@ -1,0 +1,92 @@
+"""8-bit pages and rotary positions without a GPU: the reference model itself, the frequencies, and the refusals that come before any
+device is touched."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import kv8_ref as ref
+from breccia_b200 import _lib
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_reference_encoding(code):
+    g = np.random.default_rng(1)
+    x = np.concatenate([g.uniform(-1, 1, 4000) * ref.TOP[code], g.uniform(-1, 1, 4000) * 0.05, np.arange(-200, 200) / 512.0, [0.0, 1e9, -1e9]])
+    y = ref.encode(x, code)
+    if code == "e4m3":
+        want = torch.from_numpy(np.clip(x, -448, 448)).to(torch.float32).to(torch.float8_e4m3fn).double().numpy()
+        same = x.astype(np.float32) == x   # torch rounds from f32
+        assert np.array_equal(y[same], want[same])
+    assert np.all(np.abs(y - np.clip(x, -ref.TOP[code], ref.TOP[code])) <= ref.step_of(x, code) / 2)
+    for amax in (1e-40, 0.0, 1.0, 127.0, 127.0001, 448.0, 448.1, 3e38, 2.0 ** -113 * 1.8):
+        e = ref.exponent(amax, code)
+        # the clamp: what needs more than 2^120 (int8 above 127 * 2^120) saturates
+        assert (e == 120 or amax <= ref.TOP[code] * 2.0 ** e) and (e == -120 or amax > ref.TOP[code] * 2.0 ** (e - 1))
+
+
+@pytest.mark.parametrize("scaling,more", [("none", {}), ("linear", dict(factor=4.0)), ("ntk", dict(factor=8.0)),
+                                          ("yarn", dict(factor=16.0, orig_ctx=8192)), ("bands", dict(factor=8.0, orig_ctx=8192))])
+@pytest.mark.parametrize("n_rot", [2, 64, 90, 256])
+def test_frequencies(scaling, more, n_rot):
+    from breccia_b200.qsa import Rope
+
+    rope = Rope(n_rot, theta=500000.0, scaling=scaling, **more)
+    want = ref.rope_freqs(n_rot, 500000.0, scaling, **more) / (2 * np.pi)
+    got = rope.turns_host.astype(np.float64) * 2.0 ** -64
+    # 0.64 fixed point: half of 2^-64; the reference: a few roundings of 2^-53
+    assert np.all(np.abs(got - want) <= 2.0 ** -65 + 16 * 2.0 ** -53 * want)
+    assert rope.factor == pytest.approx(0.1 * np.log(16.0) + 1 if scaling == "yarn" else 1.0, rel=2.0 ** -23)
+    assert Rope(n_rot, scaling=scaling, mscale=1.25, **more).factor == 1.25
+
+
+@pytest.mark.parametrize("bad", [dict(n_rot=3), dict(n_rot=0), dict(n_rot=258), dict(n_rot=64, theta=0.5), dict(n_rot=64, theta=float("nan")),
+                                 dict(n_rot=64, scaling="linear", factor=0.5), dict(n_rot=64, scaling="yarn", factor=2.0),
+                                 dict(n_rot=64, scaling="bands", factor=2.0, orig_ctx=8192, turns_low=4.0, turns_high=4.0),
+                                 dict(n_rot=64, mscale=-1.0), dict(n_rot=64, layout="pairs"), dict(n_rot=64, scaling="log"),
+                                 dict(n_rot=64, theta=1.0, scaling="yarn", factor=2.0, orig_ctx=8192)])
+def test_frequency_refusals(bad):
+    from breccia_b200.qsa import Rope
+
+    with pytest.raises(_lib.BrcError):
+        Rope(**bad)
+
+
+def test_rope_apply_refusals():
+    L = _lib.load()
+    d = 0x1000
+
+    def call(q=d, qo=d, nh=4, qs=0, qos=0, k=0, ko=0, nk=0, ks=0, kos=0, hd=128, dt=0, pos=d, n=3, turns=d, rot=64, lay=0):
+        return L.brc_rope_apply(0, q, qo, nh, qs, qos, k, ko, nk, ks, kos, hd, dt, pos, n, turns, rot, lay, 1.0, None)
+
+    for bad in (dict(dt=3), dict(lay=2), dict(hd=0), dict(rot=0), dict(rot=63), dict(rot=130), dict(q=0, qo=0), dict(qo=0), dict(nh=0),
+                dict(qs=511), dict(qos=511), dict(pos=0), dict(turns=0), dict(q=d + 2, qo=d + 2), dict(qo=d + 16), dict(k=d, ko=d + 512, nk=1)):
+        assert call(**bad) in (_lib.ERR_INVALID, _lib.ERR_UNSUPPORTED), bad
+    assert call(n=0) == 0
+
+
+def test_pool_refusals():
+    L = _lib.load()
+    h = C.c_void_p()
+    for args, rc in (((0, 1, 2, 256, 16, 8, 3), _lib.ERR_INVALID), ((0, 1, 2, 96, 16, 8, 1), _lib.ERR_UNSUPPORTED),
+                     ((0, 1, 2, 256, 32, 8, 1), _lib.ERR_UNSUPPORTED), ((0, 0, 2, 256, 16, 8, 2), _lib.ERR_INVALID)):
+        assert L.brc_pool_create_kv8(*args, C.byref(h)) == rc and not h.value
+    if not torch.cuda.is_available():
+        assert L.brc_pool_create_kv8(0, 1, 2, 256, 16, 8, 1, C.byref(h)) == _lib.ERR_CUDA
+    from breccia_b200.qsa import KvPool
+
+    for bad in (dict(kv8="fp8"), dict(kv8="int8", v_q8=True), dict(kv8="int8", bookkeeping_only=True)):
+        with pytest.raises(_lib.BrcError):
+            KvPool(0, 1, 2, 256, 8, **bad)
+    book = KvPool(0, 1, 2, 256, 8, bookkeeping_only=True)
+    code, b = C.c_int32(7), C.c_uint64()
+    assert L.brc_pool_kv8_code(book.handle, C.byref(code)) == 0 and code.value == 0
+    d = C.c_void_p(0x1000)
+    assert L.brc_kv8_append(book.handle, 0, d, 4, d, 1, 1, None, 1, 1, d, 0, d, 0, 0, None, 0, 0, 1.0, None) == _lib.ERR_CUDA
+    assert L.brc_kv8_read(book.handle, 0, d, 4, d, 1, 1, None, 1, 1, d, d, 0, None) == _lib.ERR_CUDA
+    assert L.brc_kv8_attn(book.handle, 0, d, 1, 16, None, 0, d, 4, d, None, 1, 1, 16, 1.0, d, 1, d, 1 << 30, None) == _lib.ERR_CUDA
+    assert L.brc_kv8_attn_workspace_bytes(book.handle, 1, 16, 1, C.byref(b)) == _lib.ERR_UNSUPPORTED
+    for null in (lambda: L.brc_kv8_append(None, 0, d, 4, d, 1, 1, None, 1, 1, d, 0, d, 0, 0, None, 0, 0, 1.0, None),
+                 lambda: L.brc_kv8_attn_workspace_bytes(None, 1, 16, 1, C.byref(b)), lambda: L.brc_pool_kv8_code(None, C.byref(code))):
+        assert null() == _lib.ERR_INVALID
