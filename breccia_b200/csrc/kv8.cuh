@@ -53,20 +53,12 @@ __device__ __forceinline__ uint32_t kv8_encode4(float a, float b, float c, float
     return q(a) | (q(b) << 8) | (q(c) << 16) | (q(d) << 24);
 }
 
-// Two codes in the low 16 bits of `w` -> two exact binary16 numbers (e4m3: every finite code is one).
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)w));
-    return r;
-}
-
-// The four codes of a word as two f16 pairs (bytes 0,1 and bytes 2,3).  int8: a byte with its sign bit flipped, under
+// The four codes of a word as two pairs of exact binary16 numbers (bytes 0,1 and bytes 2,3).  int8: a byte with its sign bit flipped, under
 // the exponent byte 0x64, is the binary16 number 1024 + 128 + code; subtracting 1152 is exact.
 template <uint32_t CODE>
 __device__ __forceinline__ void kv8_decode4(uint32_t w, uint32_t &p01, uint32_t &p23) {
     if (CODE == KV8_E4M3) {
-        p01 = e4m3x2_to_f16x2(w);
-        p23 = e4m3x2_to_f16x2(w >> 16);
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(p01), "=r"(p23) : "r"(w));
     } else {
         const uint32_t u = w ^ 0x80808080u;
         const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));   // 1152

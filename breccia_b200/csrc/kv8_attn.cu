@@ -22,9 +22,10 @@
 //     dependent launch), merges them.  No counters and no flags: nothing survives a call, so calls with workspaces of
 //     their own may overlap.
 //
-// Two running maxima per row: m of the scores s (for the sum of probabilities), and M of s + e_v, the exponent at which a
-// cell's V codes enter the result.  Weights are 2^(s + e_v - M + 15): at most 2^15, so binary16 keeps cells down to 2^-39 of
-// the heaviest one, and a page whose V scale dwarfs the others' neither overflows nor silences them.
+// Two reference exponents per row, near the running maxima: m of the scores s (for the sum of probabilities), and M of
+// s + e_v, the exponent at which a cell's V codes enter the result.  Weights are 2^(s + e_v - M + 7), below 2^15 even when a
+// score lies 2^8 over its reference, so binary16 keeps cells down to 2^-31 of the heaviest one, and a page whose V scale
+// dwarfs the others' neither overflows nor silences them.
 #include <algorithm>
 #include <atomic>
 
@@ -33,12 +34,20 @@
 
 namespace {
 
-constexpr uint32_t WARPS = 8, CONSUMERS = WARPS * 32, THREADS = CONSUMERS + 32;
+#ifndef UNIT_KIB
+#define UNIT_KIB 256u
+#endif
+#ifndef KV8_W1_128
+#define KV8_W1_128 12
+#define KV8_W1_256 8
+#define KV8_W2_128 12
+#define KV8_W2_256 8
+#endif
 constexpr uint32_t PASS_ROWS = 32;       // query rows (tokens x heads of a kv head) that share one stream of the cache
 constexpr uint32_t MIN_SHARE = 4;        // page-units a CTA takes at least
 constexpr uint32_t SMEM_LIMIT = 232448;  // 227 KiB
-constexpr uint32_t MAX_STAGES = 24;
-constexpr uint32_t SCRATCH_ROW = 132;    // floats between rows of the merge buffer: 128 and a shift of one 16-byte group
+constexpr uint32_t MAX_STAGES = 48;
+constexpr float HEADROOM = 8.f, WEIGHT_SHIFT = 7.f;   // a weight is at most 2^(WEIGHT_SHIFT + HEADROOM), half of binary16's greatest
 constexpr float NONE = -1e30f;           // running maximum before any cell
 
 struct AttnParams {
@@ -47,7 +56,7 @@ struct AttnParams {
     const float *gate;
     const uint32_t *block_tables, *seq_lens, *cu_q;
     const uint8_t *k_layer, *v_layer;
-    uint64_t *prefix;        // workspace: pages before each sequence
+    uint32_t *prefix;        // workspace: cost of the sequences before each
     float *ml;               // [slot][row of a unit][m, M, l, -]
     float *acc;              // [slot][row of a unit][head_dim]
     uint32_t *status;
@@ -55,34 +64,36 @@ struct AttnParams {
     uint32_t q_dtype, out_dtype, gate_head_stride;
     uint32_t table_stride, n_seqs, max_seq_len, max_q, n_pages, page0;   // page0: layer * n_pages
     uint32_t n_head, n_kv, group, kvb, row_groups;                        // row_groups: warps that split a pass's rows
-    uint32_t pass_rows, passes, units_per_seq, n_stages;
+    uint32_t pass_rows, passes, units_per_seq, n_stages, q_bufs, unit_cost;
     float scale_log2;
 };
 
 struct Smem {   // byte offsets behind the ring
-    uint32_t stage_bytes, q, q_lo, scratch, stat, row_fac, row_vis, bars, sched, total;
+    uint32_t stage_bytes, q, q_lo, q_bytes, scratch, stat, row_fac, row_vis, bars, sched, total;
 };
 
-__host__ __device__ inline Smem smem_layout(uint32_t hd, uint32_t kvb, uint32_t pass_rows, bool prec, uint32_t n_stages) {
+__host__ __device__ inline Smem smem_layout(uint32_t hd, uint32_t warps, uint32_t kvb, uint32_t pass_rows, bool prec, uint32_t n_stages,
+                                            uint32_t q_bufs) {
     Smem s;
     s.stage_bytes = kvb * 2u * 16u * hd;
     uint32_t at = n_stages * s.stage_bytes;
     s.q = at;
-    at += kvb * pass_rows * hd * 2u;
+    s.q_bytes = kvb * pass_rows * hd * 2u;
+    at += q_bufs * s.q_bytes;
     s.q_lo = at;
-    if (prec) at += kvb * pass_rows * hd * 2u;
-    s.scratch = at;
-    at += WARPS * 8u * SCRATCH_ROW * 4u;
-    s.stat = at;
-    at += WARPS * 16u * 4u * 4u;   // [warp][row of two tiles][m, M, l, -]
-    s.row_fac = at;
-    at += kvb * pass_rows * 4u;
-    s.row_vis = at;
-    at += pass_rows * 4u;
-    s.bars = at;
-    at += 2u * MAX_STAGES * 8u;
+    if (prec) at += q_bufs * s.q_bytes;
+    s.scratch = at;                       // [warp][row of a tile][head_dim + one 16-byte group]
+    at += warps * 8u * (hd + 4u) * 4u;
+    s.stat = at;                          // [warp][row of two tiles][m, M, l, -]
+    at += warps * 16u * 16u;
+    s.row_fac = at;                       // [buffer][head][row]
+    at += q_bufs * kvb * pass_rows * 4u;
+    s.row_vis = at;                       // [buffer][row]
+    at += q_bufs * pass_rows * 4u;
+    s.bars = at;                          // full, empty (ring); full, empty (q)
+    at += 2u * MAX_STAGES * 8u + 32u;
     s.sched = at;
-    at += 257u * 8u + 64u;
+    at += warps * 4u + 32u;
     s.total = at;
     return s;
 }
@@ -92,10 +103,10 @@ __device__ __forceinline__ uint32_t cells_of(const AttnParams &p, uint32_t s) { 
 __device__ __forceinline__ uint32_t pages_of(const AttnParams &p, uint32_t s) {
     return tokens_of(p, s) ? (cells_of(p, s) + 15u) / 16u : 0u;
 }
-__device__ __forceinline__ uint64_t share_of(uint64_t total, uint32_t grid) {
-    const uint64_t s = (total + grid - 1u) / grid;
-    return s > MIN_SHARE ? s : MIN_SHARE;
-}
+// What a unit counts for when the work is cut: its pages and, in front of them, what starting and finishing a unit costs.
+// (The host refuses a call whose costs could add up to 2^31.)
+__device__ __forceinline__ uint32_t cost_of(const AttnParams &p, uint32_t pages) { return pages ? (pages + p.unit_cost) * p.units_per_seq : 0u; }
+__device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t grid) { return max((total + grid - 1u) / grid, MIN_SHARE); }
 
 __device__ __forceinline__ void store_out(const AttnParams &p, uint64_t at, float a, float b, float c, float d) {
     if (p.out_dtype == 0) {
@@ -117,11 +128,6 @@ __device__ __forceinline__ void finish_row(const AttnParams &p, uint32_t hd, uin
     store_out(p, head_row * hd + d, v[0], v[1], v[2], v[3]);
 }
 
-__device__ __forceinline__ float4 lds128f(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-    return v;
-}
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
@@ -135,10 +141,9 @@ __device__ __forceinline__ void load_q8(const AttnParams &p, uint64_t at, float 
     else brc::load8<2>(static_cast<const __nv_bfloat16 *>(p.q) + at, true, v);
 }
 
-// A share's walk over the units: sequence, unit within it, first page.
+// A share's walk over the units: [lo, hi) on the axis of costs, and where the unit in hand begins on it.
 struct Cursor {
-    uint64_t pos, end;
-    uint32_t s, u, pg;
+    uint32_t at, lo, hi, s, u;
 };
 
 struct Segment {
@@ -146,214 +151,288 @@ struct Segment {
 };
 
 __device__ __forceinline__ bool next_segment(const AttnParams &p, Cursor &c, Segment &g) {
-    while (c.pos < c.end) {
+    while (c.at < c.hi) {
         const uint32_t pages = pages_of(p, c.s);
         if (pages == 0 || c.u == p.units_per_seq) {
             ++c.s;
-            c.u = c.pg = 0;
+            c.u = 0;
             continue;
         }
-        const uint64_t left = c.end - c.pos;
+        const uint32_t first = c.at + p.unit_cost;   // page 0's place on the axis
+        const uint32_t from = min(c.lo > first ? c.lo - first : 0u, pages), to = min(c.hi > first ? c.hi - first : 0u, pages);
         g.s = c.s;
         g.u = c.u;
-        g.pg = c.pg;
         g.pages = pages;
-        g.n = (uint32_t)(pages - c.pg < left ? pages - c.pg : left);
-        c.pos += g.n;
-        c.pg = 0;
+        g.pg = from;
+        g.n = to > from ? to - from : 0u;
+        c.at = first + pages;
         ++c.u;
-        return true;
+        if (g.n) return true;   // a share may end inside a unit's cost, in front of its first page
     }
     return false;
 }
 
-// RT: tiles of eight query rows that a warp carries.  PREC: q and the probabilities as two binary16 parts each.
-template <int HD, uint32_t CODE, bool PREC, int RT>
-__global__ void __launch_bounds__(THREADS, 1) kv8_attn_kernel(const __grid_constant__ CUtensorMap tm, const AttnParams p) {
-    constexpr uint32_t SLABS = HD / 128;
+// q rows of a unit, scaled by a power of two to at most 2^15 in magnitude and laid out as the B fragments of the K product:
+// [8-row tile][pair of 16-column steps][lane][2 x 4 values]; column d belongs to step 8 (d / 128) + 4 (d / 16 % 2) +
+// d / 4 % 4 and thread d / 32 % 4 of its row's group.  A row takes HD / 8 lanes; warp `w` of `n_w` has every n_w-th set of
+// 256 / HD rows, U sets of loads in flight; `meanwhile` runs behind the first loads.
+template <int HD, bool PREC, int U, class F>
+__device__ __forceinline__ void stage_q(const AttnParams &p, const Smem &L, uint8_t *smem, const Segment &g, uint32_t buf, uint32_t w,
+                                        uint32_t n_w, uint32_t lane, F &&meanwhile) {
+    constexpr uint32_t LANES = HD / 8, SET = 32 / LANES;
+    const uint32_t hg = g.u / p.passes, pass = g.u % p.passes;
+    const uint32_t n_q = tokens_of(p, g.s), len = cells_of(p, g.s);
+    const uint64_t tok0 = p.cu_q ? p.cu_q[g.s] : (uint64_t)g.s * p.max_q;
+    const uint32_t rows = min(n_q, p.max_q) * p.group, all = p.kvb * p.pass_rows, d = lane % LANES * 8u;
+    float *row_fac = reinterpret_cast<float *>(smem + L.row_fac) + buf * all;
+    uint32_t *row_vis = reinterpret_cast<uint32_t *>(smem + L.row_vis) + buf * p.pass_rows;
+    for (uint32_t r0 = w * SET + lane / LANES; r0 / SET * SET < all; r0 += n_w * SET * U) {   // (all is a multiple of SET: whole warps)
+        float v[U][8];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const uint32_t rr = r0 + k * n_w * SET, h = rr / p.pass_rows, gr_row = pass * p.pass_rows + rr % p.pass_rows;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
+            if (rr < all && gr_row < rows)
+                load_q8(p, ((tok0 + gr_row / p.group) * p.n_head + (hg * p.kvb + h) * p.group + gr_row % p.group) * HD + d, v[k]);
+        }
+        if (r0 < n_w * SET) meanwhile();
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const uint32_t rr = r0 + k * n_w * SET;
+            if (rr >= all) break;
+            const uint32_t h = rr / p.pass_rows, r = rr % p.pass_rows, gr_row = pass * p.pass_rows + r;
+            float amax = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[k][i]));
+#pragma unroll
+            for (int m = LANES / 2; m; m >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
+            const int ex = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 127);
+            const float up = brc::exp2_int(14 - ex);
+            if (d == 0) {
+                row_fac[rr] = amax <= 3.402823466e38f ? brc::exp2_int(ex - 14) * p.scale_log2 : __uint_as_float(0x7fffffffu);
+                if (h == 0) {   // cells that the row sees; rows of no token: like the last token's
+                    const uint32_t tok = gr_row / p.group;
+                    row_vis[r] = gr_row >= rows ? len : len + tok + 1u > n_q ? len + tok + 1u - n_q : 0u;
+                }
+            }
+            const uint32_t step = 8u * (d / 128u) + 4u * (d / 16u % 2u) + d / 4u % 4u;   // of the first four values; the next four: step + 1
+            const uint32_t at = buf * L.q_bytes + (h * p.pass_rows + r / 8u * 8u) * HD * 2u +
+                                ((step / 2u) * 32u + (r % 8u) * 4u + d / 32u % 4u) * 16u;
+            uint32_t a[4], b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = v[k][2 * i] * up, y = v[k][2 * i + 1] * up;
+                a[i] = brc::pack_half2(x, y);
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&a[i]));
+                b[i] = brc::pack_half2(x - f.x, y - f.y);
+            }
+            *reinterpret_cast<uint4 *>(smem + L.q + at) = make_uint4(a[0], a[1], a[2], a[3]);
+            if (PREC) *reinterpret_cast<uint4 *>(smem + L.q_lo + at) = make_uint4(b[0], b[1], b[2], b[3]);
+        }
+    }
+}
+
+// RT: tiles of eight query rows that a warp carries; W: consuming warps.  PREC: q and the probabilities as two binary16 parts each.
+template <int HD, uint32_t CODE, bool PREC, int RT, int W>
+__global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_constant__ CUtensorMap tm, const AttnParams p) {
+    constexpr uint32_t SLABS = HD / 128, CONSUMERS = W * 32, ROW = HD + 4;
     extern __shared__ __align__(1024) uint8_t smem[];
-    const Smem L = smem_layout(HD, p.kvb, p.pass_rows, PREC, p.n_stages);
+    const Smem L = smem_layout(HD, W, p.kvb, p.pass_rows, PREC, p.n_stages, p.q_bufs);
     const uint32_t base = brc::smem_u32(smem);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-    const uint32_t full0 = base + L.bars, empty0 = full0 + MAX_STAGES * 8u;
-    uint64_t *chunk_prefix = reinterpret_cast<uint64_t *>(smem + L.sched);   // [257]: pages before each thread's sequences
-    Cursor *cursor = reinterpret_cast<Cursor *>(smem + L.sched + 257u * 8u);
+    const uint32_t full0 = base + L.bars, empty0 = full0 + MAX_STAGES * 8u, q_full0 = empty0 + MAX_STAGES * 8u, q_empty0 = q_full0 + 16u;
+    uint32_t *warp_cost = reinterpret_cast<uint32_t *>(smem + L.sched);   // [W]: cost of each warp's sequences
+    Cursor *cursor = reinterpret_cast<Cursor *>(smem + L.sched + W * 4u);
+    if (tid == CONSUMERS) {
+        for (uint32_t i = 0; i < p.n_stages; ++i) {
+            brc::mbar_init(full0 + 8u * i, 1u);
+            brc::mbar_init(empty0 + 8u * i, p.kvb * p.row_groups);       // the warps that read a stage
+        }
+        for (uint32_t i = 0; i < p.q_bufs; ++i) {
+            brc::mbar_init(q_full0 + 8u * i, 3u);                        // helper warps
+            brc::mbar_init(q_empty0 + 8u * i, W);
+        }
+        brc::mbar_fence_init();
+        brc::tma_prefetch_desc(&tm);
+    }
+    // Everything up to here may overlap the end of the kernel in front of this one; what it wrote is read from here on.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    // ---- the cut: pages of all sequences, summed by 256 threads over equal runs of sequences
+    // ---- the cut: costs of all sequences, summed by the consumers over equal runs of sequences
     const uint32_t per_thread = (p.n_seqs + CONSUMERS - 1u) / CONSUMERS;
+    uint32_t sum = 0, run = 0;
     if (tid < CONSUMERS) {
-        uint64_t sum = 0;
         for (uint32_t i = 0; i < per_thread; ++i) {
             const uint32_t s = tid * per_thread + i;
             if (s >= p.n_seqs) break;
-            sum += pages_of(p, s);
+            sum += cost_of(p, pages_of(p, s));
             if (blockIdx.x == 0) {
                 if (p.seq_lens[s] > p.max_seq_len) { atomicOr(p.status, BRC_DEV_BAD_POS); p.status[1] = p.seq_lens[s]; }
                 if (tokens_of(p, s) > p.max_q) { atomicOr(p.status, BRC_DEV_BAD_POS); p.status[1] = tokens_of(p, s); }
             }
         }
-        uint64_t run = sum;
+        run = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t up = __shfl_up_sync(0xffffffffu, run, o);
+            const uint32_t up = __shfl_up_sync(0xffffffffu, run, o);
             if (lane >= (uint32_t)o) run += up;
         }
-        chunk_prefix[tid + 1] = run;   // within the warp, for now
-        if (tid == 0) chunk_prefix[0] = 0;
+        if (lane == 31u) warp_cost[warp] = run;
     }
-    if (tid == CONSUMERS) {
-        const uint32_t users = p.kvb * p.row_groups;
-        for (uint32_t i = 0; i < p.n_stages; ++i) {
-            brc::mbar_init(full0 + 8u * i, 1u);
-            brc::mbar_init(empty0 + 8u * i, users);
+    __syncthreads();
+    uint32_t before = 0, total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w) {
+        before += w < warp ? warp_cost[w] : 0u;
+        total += warp_cost[w];
+    }
+    const uint32_t share = share_of(total, gridDim.x), lo = min(total, blockIdx.x * share), hi = min(total, lo + share);
+    if (tid < CONSUMERS) {
+        uint32_t at = before + run - sum;   // cost in front of this thread's sequences
+        if (lo < hi && at <= lo && lo < at + sum) {
+            uint32_t a = at, c;
+            uint32_t s = tid * per_thread;
+            while (a + (c = cost_of(p, pages_of(p, s))) <= lo) {
+                a += c;
+                ++s;
+            }
+            c /= p.units_per_seq;
+            const uint32_t u = (lo - a) / c;
+            *cursor = Cursor{a + u * c, lo, hi, s, u};
         }
-        brc::mbar_fence_init();
-        brc::tma_prefetch_desc(&tm);
-    }
-    __syncthreads();
-    uint64_t before = 0;
-    if (tid < CONSUMERS)
-        for (uint32_t w = 0; w < warp; ++w) before += chunk_prefix[w * 32u + 32u];
-    __syncthreads();
-    if (tid < CONSUMERS) chunk_prefix[tid + 1] += before;
-    __syncthreads();
-    const uint64_t total = chunk_prefix[CONSUMERS] * p.units_per_seq;
-    const uint64_t share = share_of(total, gridDim.x);
-    const uint64_t lo = min(total, blockIdx.x * share), hi = min(total, lo + share);
-    if (blockIdx.x == 0 && tid < CONSUMERS) {   // for the merging kernel
-        uint64_t at = chunk_prefix[tid];
-        if (tid == 0) p.prefix[0] = 0;
-        for (uint32_t i = 0; i < per_thread; ++i) {
-            const uint32_t s = tid * per_thread + i;
-            if (s >= p.n_seqs) break;
-            at += pages_of(p, s);
-            p.prefix[s + 1] = at;
+        if (blockIdx.x == 0) {   // for the merging kernel
+            if (tid == 0) p.prefix[0] = 0;
+            for (uint32_t i = 0; i < per_thread; ++i) {
+                const uint32_t s = tid * per_thread + i;
+                if (s >= p.n_seqs) break;
+                at += cost_of(p, pages_of(p, s));
+                p.prefix[s + 1] = at;
+            }
         }
     }
     if (lo >= hi) return;
-    if (tid == 0) {
-        uint32_t a = 0, b = CONSUMERS;   // last run of sequences that begins at or before lo and holds pages behind it
-        while (b - a > 1u) {
-            const uint32_t mid = (a + b) >> 1;
-            if (chunk_prefix[mid] * p.units_per_seq <= lo) a = mid; else b = mid;
-        }
-        uint64_t at = chunk_prefix[a] * p.units_per_seq;
-        uint32_t s = a * per_thread;
-        uint32_t pages;
-        while (true) {
-            pages = pages_of(p, s);
-            if (at + (uint64_t)pages * p.units_per_seq > lo) break;
-            at += (uint64_t)pages * p.units_per_seq;
-            ++s;
-        }
-        cursor->pos = lo;
-        cursor->end = hi;
-        cursor->s = s;
-        cursor->u = (uint32_t)((lo - at) / pages);
-        cursor->pg = (uint32_t)((lo - at) % pages);
-    }
     __syncthreads();
     Cursor cur = *cursor;
     Segment g;
 
-    if (warp == WARPS) {
-        // ------------------------------------------------------------------ producer: one page-unit per stage
-        const uint64_t policy = brc::l2_policy_evict_first();
-        uint32_t stage = 0, parity = 1;   // the first round finds every stage empty
+    // Registers: launched with 168 / 128 / 96 a thread (8 / 12 / 16 consuming warps and four more), of which the four others
+    // keep 56 and hand the rest to the consumers; the sums stay within what the block was launched with.
+    if (warp >= W) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         bool ok = true;
-        while (ok && next_segment(p, cur, g)) {
-            const uint32_t row = (g.u / p.passes) * p.kvb * 16u;
-            const uint32_t *table = p.block_tables + (uint64_t)g.s * p.table_stride + g.pg;
-            uint32_t ahead = lane < g.n ? table[lane] : 0u;
-            for (uint32_t i0 = 0; ok && i0 < g.n; i0 += 32u) {
-                const uint32_t ids = ahead;
-                if (i0 + 32u + lane < g.n) ahead = table[i0 + 32u + lane];
-                const uint32_t m = min(32u, g.n - i0);
-                for (uint32_t i = 0; i < m; ++i) {
-                    uint32_t id = __shfl_sync(0xffffffffu, ids, i);
-                    if (id >= p.n_pages) id = 0;   // the consumers report it and mask the cells
-                    ok = brc::mbar_wait(empty0 + 8u * stage, parity);
+        if (warp > W) {
+            // -------------------------------------------------------------- helpers: q of every unit but the first
+            uint32_t idx = 0;
+            while (next_segment(p, cur, g)) {
+                if (idx) {
+                    const uint32_t buf = idx % p.q_bufs;
+                    if (idx >= p.q_bufs) ok = brc::mbar_wait(q_empty0 + 8u * buf, (idx - p.q_bufs) / p.q_bufs & 1u);
                     if (!ok) break;
-                    if (lane == 0) {
-                        brc::mbar_arrive_expect_tx(full0 + 8u * stage, L.stage_bytes);
-#pragma unroll
-                        for (uint32_t sl = 0; sl < SLABS; ++sl)
-                            brc::tma_load_4d(base + stage * L.stage_bytes + sl * (L.stage_bytes / SLABS), &tm, (int32_t)(sl * 128u), (int32_t)row,
-                                             (int32_t)(p.page0 + id), 0, full0 + 8u * stage, policy);
+                    stage_q<HD, PREC, 2>(p, L, smem, g, buf, warp - W - 1u, 3u, lane, [] {});
+                    __syncwarp();
+                    if (lane == 0) brc::mbar_arrive(q_full0 + 8u * buf);
+                }
+                ++idx;
+            }
+        } else {
+            // -------------------------------------------------------------- producer: one page-unit per stage, four boxes at a time,
+            // a lane each (one lane alone takes 390 clocks for wait, arrival and box; the stream wants a stage of 8 KiB every 345)
+            constexpr uint32_t BATCH = 4 / SLABS;   // stages of a round
+            const uint64_t policy = brc::l2_policy_evict_first();
+            const uint32_t j = lane / SLABS, sl = lane % SLABS;
+            uint32_t stage = 0, parity = 1;   // the first round finds every stage empty
+            while (ok && next_segment(p, cur, g)) {
+                const uint32_t row0 = (g.u / p.passes) * p.kvb * 16u;
+                const uint32_t *table = p.block_tables + (uint64_t)g.s * p.table_stride + g.pg;
+                uint32_t ahead = lane < g.n ? table[lane] : 0u;
+                for (uint32_t i0 = 0; ok && i0 < g.n; i0 += 32u) {
+                    const uint32_t ids = ahead;
+                    if (i0 + 32u + lane < g.n) ahead = table[i0 + 32u + lane];
+                    const uint32_t m = min(32u, g.n - i0);
+                    for (uint32_t i = 0; ok && i < m; i += BATCH) {
+                        uint32_t id = __shfl_sync(0xffffffffu, ids, (i + j) & 31u);
+                        if (id >= p.n_pages) id = 0;   // the consumers report it and mask the cells
+                        const bool mine = j < BATCH && i + j < m;
+                        const bool wrap = stage + j >= p.n_stages;
+                        const uint32_t st = wrap ? stage + j - p.n_stages : stage + j;
+                        if (mine) {
+                            ok = brc::mbar_wait(empty0 + 8u * st, wrap ? parity ^ 1u : parity);
+                            if (ok && sl == 0) brc::mbar_arrive_expect_tx(full0 + 8u * st, L.stage_bytes);
+                        }
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (mine && ok)
+                            brc::tma_load_4d(base + st * L.stage_bytes + sl * (L.stage_bytes / SLABS), &tm, (int32_t)(sl * 128u), (int32_t)row0,
+                                             (int32_t)(p.page0 + id), 0, full0 + 8u * st, policy);
+                        stage += min(BATCH, m - i);
+                        if (stage >= p.n_stages) { stage -= p.n_stages; parity ^= 1u; }
                     }
-                    if (++stage == p.n_stages) { stage = 0; parity ^= 1u; }
                 }
             }
         }
         if (!ok && lane == 0) { atomicOr(p.status, BRC_DEV_WAIT_LIMIT); p.status[1] = blockIdx.x; }
         return;
     }
+    if constexpr (W == 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    else if constexpr (W == 12) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
 
     // ---------------------------------------------------------------------- consumers
     const uint32_t t = lane & 3u, gr = lane >> 2;            // thread of a group, group
     const uint32_t hk = warp % p.kvb, rg = warp / p.kvb % p.row_groups;
-    const uint32_t lanes = WARPS / (p.kvb * p.row_groups);   // warps that take pages in turn
+    const uint32_t lanes = W / (p.kvb * p.row_groups);   // warps that take pages in turn
     const uint32_t pl = warp / (p.kvb * p.row_groups);
     const uint32_t slab_bytes = p.kvb * 2u * 16u * 128u;     // [K|V][head][cell][128]
     float *scratch = reinterpret_cast<float *>(smem + L.scratch);
     float4 *stat = reinterpret_cast<float4 *>(smem + L.stat);
-    float *row_fac = reinterpret_cast<float *>(smem + L.row_fac);
-    uint32_t *row_vis = reinterpret_cast<uint32_t *>(smem + L.row_vis);
-    const uint32_t q_frag = base + L.q + (hk * p.pass_rows + rg * RT * 8u) * HD * 2u + lane * 16u;
-    const uint32_t q_frag_lo = base + L.q_lo + (hk * p.pass_rows + rg * RT * 8u) * HD * 2u + lane * 16u;
     const uint64_t code_bytes = (uint64_t)p.n_kv * 16u * HD;
-    uint32_t done = 0;   // page-units of the segments before this one
+    // Scales of this warp's next 32 page-units of a segment, one a lane, in two steps so that nobody waits for a page id:
+    // ids_of asks for the ids, scales_of some time later for the scales.  An id out of range shows as a negative scale.
+    auto ids_of = [&](const Segment &g, uint32_t i0) {
+        const uint32_t i = i0 + lanes * lane;
+        return i < g.n ? p.block_tables[(uint64_t)g.s * p.table_stride + g.pg + i] : 0u;
+    };
+    auto scales_of = [&](const Segment &g, uint32_t id, float &ks, float &vs) {
+        if (id < p.n_pages) {
+            const uint64_t at = id * p.page_bytes + code_bytes + (g.u / p.passes * p.kvb + hk) * 4u;
+            ks = *reinterpret_cast<const float *>(p.k_layer + at);
+            vs = *reinterpret_cast<const float *>(p.v_layer + at);
+        } else {
+            ks = vs = -1.f;
+            atomicOr(p.status, BRC_DEV_BAD_PAGE);
+            p.status[1] = id;
+        }
+    };
+    uint32_t stage = pl, parity = 0;   // of this warp's next page-unit
+    uint32_t done = 0, idx = 0;   // page-units and units of the segments before this one
     bool ok = true;
 
-    while (next_segment(p, cur, g)) {
+    Segment g_next;
+    bool more = next_segment(p, cur, g);
+    uint32_t ids = more ? ids_of(g, pl) : 0u;
+    while (more) {
         const uint32_t hg = g.u / p.passes, pass = g.u % p.passes;
         const uint32_t n_q = tokens_of(p, g.s), len = cells_of(p, g.s);
         const uint64_t tok0 = p.cu_q ? p.cu_q[g.s] : (uint64_t)g.s * p.max_q;
-        const uint32_t rows = min(n_q, p.max_q) * p.group;   // of a kv head, over all passes
-
-        // q rows of this unit, scaled by a power of two to at most 2^15 in magnitude and laid out as the B fragments of the
-        // K product: [8-row tile][pair of 16-column steps][lane][2 x 4 values]; column d belongs to step
-        // 8 (d / 128) + 4 (d / 16 % 2) + d / 4 % 4 and thread d / 32 % 4 of its row's group.
-        for (uint32_t r0 = warp; r0 < p.kvb * p.pass_rows; r0 += WARPS) {
-            const uint32_t h = r0 / p.pass_rows, r = r0 % p.pass_rows, gr_row = pass * p.pass_rows + r;
-            const bool live = gr_row < rows;
-            const uint32_t tok = gr_row / p.group, head = (hg * p.kvb + h) * p.group + gr_row % p.group;
-            const uint32_t d = lane * 8u;
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.f;
-            if (live && d < HD) load_q8(p, ((tok0 + tok) * p.n_head + head) * HD + d, v);
-            float amax = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
-#pragma unroll
-            for (int m = 16; m; m >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
-            const int ex = max((int)(__float_as_uint(amax) >> 23) - 127, -100);
-            const float up = brc::exp2_int(14 - min(ex, 127));
-            if (lane == 0) {
-                row_fac[r0] = amax <= 3.402823466e38f ? brc::exp2_int(ex - 14) * p.scale_log2 : __uint_as_float(0x7fffffffu);
-                if (h == 0) row_vis[r] = live && len + tok + 1u > n_q ? len + tok + 1u - n_q : 0u;
-            }
-            if (d < HD) {
-                const uint32_t tile = r / 8u, step = 8u * (d / 128u) + 4u * (d / 16u % 2u) + d / 4u % 4u;   // of the first four; the next four are step + 1
-                const uint32_t frag_lane = (r % 8u) * 4u + d / 32u % 4u;
-                const uint32_t at = (h * p.pass_rows + tile * 8u) * HD * 2u + ((step / 2u) * 32u + frag_lane) * 16u;
-                float hi16[8], lo16[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = v[i] * up;
-                    hi16[i] = __half2float(__float2half_rn(x));
-                    lo16[i] = x - hi16[i];
-                }
-                *reinterpret_cast<uint4 *>(smem + L.q + at) = make_uint4(brc::pack_half2(hi16[0], hi16[1]), brc::pack_half2(hi16[2], hi16[3]),
-                                                                         brc::pack_half2(hi16[4], hi16[5]), brc::pack_half2(hi16[6], hi16[7]));
-                if (PREC)
-                    *reinterpret_cast<uint4 *>(smem + L.q_lo + at) = make_uint4(brc::pack_half2(lo16[0], lo16[1]), brc::pack_half2(lo16[2], lo16[3]),
-                                                                                brc::pack_half2(lo16[4], lo16[5]), brc::pack_half2(lo16[6], lo16[7]));
-            }
+        const uint32_t rows = min(n_q, p.max_q) * p.group;               // of a kv head, over all passes
+        const uint32_t vis_min = len + 1u > n_q ? len + 1u - n_q : 0u;   // cells that every row sees
+        const uint32_t buf_q = idx % p.q_bufs;
+        float ks_now = 1.f, vs_now = 1.f, ks_next = 1.f, vs_next = 1.f;
+        if (idx == 0) {   // the first unit's q: nobody has anything else to do yet
+            // (scales asked for with the q rows: behind the first pages' boxes they would come 3 us later)
+            bool asked = false;
+            stage_q<HD, PREC, 2>(p, L, smem, g, 0, warp, W, lane, [&] { scales_of(g, ids, ks_next, vs_next); asked = true; });
+            if (!asked) scales_of(g, ids, ks_next, vs_next);
+            brc::named_bar_sync(1, CONSUMERS);
+        } else {
+            scales_of(g, ids, ks_next, vs_next);
+            ok = ok && brc::mbar_wait(q_full0 + 8u * buf_q, (idx - 1u) / p.q_bufs & 1u);
         }
-        brc::named_bar_sync(1, CONSUMERS);
+        const float *row_fac = reinterpret_cast<const float *>(smem + L.row_fac) + (buf_q * p.kvb + hk) * p.pass_rows;
+        const uint32_t *row_vis = reinterpret_cast<const uint32_t *>(smem + L.row_vis) + buf_q * p.pass_rows;
+        const uint32_t q_at = buf_q * L.q_bytes + (hk * p.pass_rows + rg * RT * 8u) * HD * 2u + lane * 16u;
+        const uint32_t q_frag = base + L.q + q_at, q_frag_lo = base + L.q_lo + q_at;
 
         float o[RT][SLABS * 8][4];
         float m_run[RT][2], w_run[RT][2], l_run[RT][2], fac[RT][2];
@@ -369,45 +448,21 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attn_kernel(const __grid_const
                 const uint32_t r = (rg * RT + n) * 8u + 2u * t + i;
                 m_run[n][i] = w_run[n][i] = NONE;
                 l_run[n][i] = 0.f;
-                fac[n][i] = row_fac[hk * p.pass_rows + r];
+                fac[n][i] = row_fac[r];
                 vis[n][i] = row_vis[r];
             }
         }
 
-        // scales of this warp's next 32 page-units, one a lane, fetched a batch ahead; a page id out of range shows as a
-        // negative scale
-        const uint32_t *table = p.block_tables + (uint64_t)g.s * p.table_stride + g.pg;
-        const uint32_t first = (pl + lanes - done % lanes) % lanes;
-        auto fetch = [&](uint32_t i0, float &ks, float &vs) {
-            const uint32_t i = i0 + lanes * lane;
-            ks = vs = 1.f;
-            if (i < g.n) {
-                const uint32_t id = table[i];
-                if (id < p.n_pages) {
-                    const uint64_t at = id * p.page_bytes + code_bytes + (hg * p.kvb + hk) * 4u;
-                    ks = *reinterpret_cast<const float *>(p.k_layer + at);
-                    vs = *reinterpret_cast<const float *>(p.v_layer + at);
-                } else {
-                    ks = -1.f;
-                    atomicOr(p.status, BRC_DEV_BAD_PAGE);
-                    p.status[1] = id;
-                }
-            }
-        };
-        float ks_now, vs_now, ks_next = 1.f, vs_next = 1.f;
-        fetch(first, ks_next, vs_next);
-        ks_now = ks_next;
-        vs_now = vs_next;
-
-        for (uint32_t i = first, k = 0; i < g.n; i += lanes, ++k) {
+        for (uint32_t i = (pl + lanes - done % lanes) % lanes, k = 0; i < g.n; i += lanes, ++k) {
             if (k % 32u == 0u) {
                 ks_now = ks_next;
                 vs_now = vs_next;
-                fetch(i + lanes * 32u, ks_next, vs_next);
+                ids = ids_of(g, i + lanes * 32u);
+            } else if (k % 32u == 16u) {
+                scales_of(g, ids, ks_next, vs_next);
             }
             const float ks = __shfl_sync(0xffffffffu, ks_now, k % 32u), vs = __shfl_sync(0xffffffffu, vs_now, k % 32u);
-            const uint32_t unit = done + i, stage = unit % p.n_stages;
-            ok = ok && brc::mbar_wait(full0 + 8u * stage, unit / p.n_stages & 1u);
+            ok = ok && brc::mbar_wait(full0 + 8u * stage, parity);
             if (!ok) break;   // the producer gave up or its copy never came: no further wait, the sums stay as they are
             const uint32_t buf = base + stage * L.stage_bytes;
             const uint32_t cell0 = (g.pg + i) * 16u;
@@ -453,32 +508,41 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attn_kernel(const __grid_const
                     for (int x = 0; x < 4; ++x) s[n][x] = part[n][0][x] + part[n][1][x];
             }
 
-            // ---- softmax over the running maxima; weights to B fragments [cells][rows]
+            // ---- softmax against the rows' reference exponents; weights to B fragments [cells][rows].  The references
+            // move only when a score passes one by more than 2^HEADROOM, so an ordinary page needs no maximum across the warp.
             const bool good = ks > 0.f;
             const float ev = (float)brc::kv8_scale_exponent(vs);
+            const bool edge = cell0 + 16u > vis_min || !good;
             uint32_t pw[RT][2], pw_lo[RT][2];
 #pragma unroll
             for (int n = 0; n < RT; ++n) {
-                float f[2], wt[4];
+                float wt[4];
+                bool over = false;
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {   // the thread's two rows: cells gr and gr + 8
                     const float kf = fac[n][x] * ks;
-                    const bool see0 = good && cell0 + gr < vis[n][x], see1 = good && cell0 + gr + 8u < vis[n][x];
-                    const float s0 = see0 ? s[n][x] * kf : -INFINITY, s1 = see1 ? s[n][x + 2] * kf : -INFINITY;
-                    float top = fmaxf(s0, s1);
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const float m_new = fmaxf(m_run[n][x], top), w_new = fmaxf(w_run[n][x], top + ev);
-                    l_run[n][x] = l_run[n][x] * brc::fast_exp2(m_run[n][x] - m_new) + (brc::fast_exp2(s0 - m_new) + brc::fast_exp2(s1 - m_new));
-                    f[x] = brc::fast_exp2(w_run[n][x] - w_new);
-                    const float shift = ev - w_new + 15.f;
-                    wt[x] = brc::fast_exp2(s0 + shift);
-                    wt[x + 2] = brc::fast_exp2(s1 + shift);
-                    m_run[n][x] = m_new;
-                    w_run[n][x] = w_new;
+                    s[n][x] *= kf;
+                    s[n][x + 2] *= kf;
+                    if (edge) {
+                        if (!good || cell0 + gr >= vis[n][x]) s[n][x] = -INFINITY;
+                        if (!good || cell0 + gr + 8u >= vis[n][x]) s[n][x + 2] = -INFINITY;
+                    }
+                    over |= fmaxf(s[n][x], s[n][x + 2]) > fminf(m_run[n][x], w_run[n][x] - ev) + HEADROOM;
                 }
-                if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+                if (__any_sync(0xffffffffu, over)) {
+                    float f[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float top = fmaxf(s[n][x], s[n][x + 2]);
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        const float m_new = fmaxf(m_run[n][x], top), w_new = fmaxf(w_run[n][x], top + ev);
+                        l_run[n][x] *= brc::fast_exp2(m_run[n][x] - m_new);
+                        f[x] = brc::fast_exp2(w_run[n][x] - w_new);
+                        m_run[n][x] = m_new;
+                        w_run[n][x] = w_new;
+                    }
 #pragma unroll
                     for (int j = 0; j < (int)SLABS * 8; ++j) {
                         o[n][j][0] *= f[0];
@@ -486,6 +550,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attn_kernel(const __grid_const
                         o[n][j][2] *= f[0];
                         o[n][j][3] *= f[1];
                     }
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const float shift = ev - w_run[n][x] + WEIGHT_SHIFT;
+                    l_run[n][x] += brc::fast_exp2(s[n][x] - m_run[n][x]) + brc::fast_exp2(s[n][x + 2] - m_run[n][x]);
+                    wt[x] = brc::fast_exp2(s[n][x] + shift);
+                    wt[x + 2] = brc::fast_exp2(s[n][x + 2] + shift);
                 }
                 const uint32_t a = brc::pack_half2(wt[0], wt[1]), b = brc::pack_half2(wt[2], wt[3]);
                 pw[n][0] = brc::movmatrix_trans(a);
@@ -540,8 +611,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attn_kernel(const __grid_const
             }
             __syncwarp();
             if (lane == 0) brc::mbar_arrive(empty0 + 8u * stage);
+            stage += lanes;
+            if (stage >= p.n_stages) { stage -= p.n_stages; parity ^= 1u; }   // (n_stages is a multiple of lanes)
         }
         done += g.n;
+        __syncwarp();
+        if (lane == 0) brc::mbar_arrive(q_empty0 + 8u * buf_q);
+        ++idx;
 
         // ---- merge the warps that took this unit's pages in turn; finish it, or leave a partial
 #pragma unroll
@@ -556,24 +632,28 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attn_kernel(const __grid_const
             }
         const bool whole = g.n == g.pages;
         const uint64_t slot = 2ull * blockIdx.x + (g.pg == 0 ? 1u : 0u);
+        more = next_segment(p, cur, g_next);
+        if (more) ids = ids_of(g_next, (pl + lanes - done % lanes) % lanes);   // on their way while this unit is merged
 #pragma unroll
         for (int n = 0; n < RT; ++n) {
 #pragma unroll
-            for (uint32_t sl = 0; sl < SLABS; ++sl) {
+            for (uint32_t sl = 0; sl < SLABS; ++sl)
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
-                    for (uint32_t x = 0; x < 2; ++x)
+                    for (uint32_t y = 0; y < 2; ++y)
 #pragma unroll
-                        for (uint32_t y = 0; y < 2; ++y) {
+                        for (uint32_t x = 0; x < 2; ++x) {
                             const float(*a)[4] = &o[n][sl * 8u + 4u * y];
-                            *reinterpret_cast<float4 *>(scratch + (warp * 8u + 2u * t + x) * SCRATCH_ROW + 16u * gr + 8u * h + 4u * y) =
+                            *reinterpret_cast<float4 *>(scratch + (warp * 8u + 2u * t + x) * ROW + 128u * sl + 16u * gr + 8u * h + 4u * y) =
                                 make_float4(a[0][2 * h + x], a[1][2 * h + x], a[2][2 * h + x], a[3][2 * h + x]);
                         }
-                brc::named_bar_sync(1, CONSUMERS);
-                const uint32_t items = p.kvb * p.row_groups * 8u * 32u;
+            brc::named_bar_sync(1, CONSUMERS);
+            {
+                constexpr uint32_t C4 = HD / 4;
+                const uint32_t items = p.kvb * p.row_groups * 8u * C4;
                 for (uint32_t it = tid; it < items; it += CONSUMERS) {
-                    const uint32_t c4 = it % 32u, row8 = it / 32u % 8u, wg = it / 256u;   // wg = head + kvb * row group
+                    const uint32_t d = it % C4 * 4u, row8 = it / C4 % 8u, wg = it / (8u * C4);   // wg = head + kvb * row group
                     const uint32_t r = ((wg / p.kvb) * RT + n) * 8u + row8, h = wg % p.kvb;
                     const uint32_t gr_row = pass * p.pass_rows + r;
                     if (gr_row >= rows) continue;
@@ -589,15 +669,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attn_kernel(const __grid_const
                         const float4 st = stat[w * 16u + n * 8u + row8];
                         l += st.z * brc::fast_exp2(st.x - m);
                         const float f = brc::fast_exp2(st.y - wm);
-                        const float4 x = lds128f(base + L.scratch + ((w * 8u + row8) * SCRATCH_ROW + c4 * 4u) * 4u);
+                        const float4 x = *reinterpret_cast<const float4 *>(scratch + (w * 8u + row8) * ROW + d);
                         v[0] += x.x * f;
                         v[1] += x.y * f;
                         v[2] += x.z * f;
                         v[3] += x.w * f;
                     }
-                    const uint32_t d = sl * 128u + c4 * 4u;
                     if (whole) {
-                        const float f = l == 0.f ? 0.f : brc::fast_exp2(wm - m - 15.f) / l;
+                        const float f = l == 0.f ? 0.f : brc::fast_exp2(wm - m - WEIGHT_SHIFT) / l;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) v[e] *= f;
                         const uint32_t tok = gr_row / p.group, head = (hg * p.kvb + h) * p.group + gr_row % p.group;
@@ -611,78 +690,113 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attn_kernel(const __grid_const
                 brc::named_bar_sync(1, CONSUMERS);
             }
         }
+        g = g_next;
     }
     if (!ok && lane == 0) { atomicOr(p.status, BRC_DEV_WAIT_LIMIT); p.status[1] = blockIdx.x; }
 }
 
-// One CTA per (unit, query row): the partials that the shares' boundaries left of it, in share order; zeros for a sequence
-// without cells.  Units that one share covered are finished already.
-template <int HD>
-__global__ void __launch_bounds__(256) kv8_merge_kernel(const AttnParams p, uint32_t grid) {
+// The partials that the shares' boundaries left of each (unit, query row), merged in share order; zeros for a sequence without
+// cells.  Units that one share covered are finished already.  W warps per row, ROWS rows per CTA, B partials of a warp
+// in flight (their sums and exponents together: one round trip).
+template <int HD, int W, int ROWS, int B>
+__global__ void __launch_bounds__(W * ROWS * 32) kv8_merge_kernel(const AttnParams p, uint32_t grid) {
     constexpr uint32_t PER = HD / 32;
+    __shared__ float part[W == 1 ? 1 : W][HD];
+    __shared__ float4 warp_stat[W];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    __shared__ float part[8][HD];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t s = blockIdx.x / p.units_per_seq, u = blockIdx.x % p.units_per_seq;
-    const uint64_t before = p.prefix[s], pages = p.prefix[s + 1] - before;
-    const uint64_t share = share_of(p.prefix[p.n_seqs] * p.units_per_seq, grid);
-    const uint64_t begin = before * p.units_per_seq + u * pages;
-    const uint64_t c0 = begin / share, c1 = pages ? (begin + pages - 1u) / share : c0;
-    if (pages && c0 == c1) return;
-    const uint32_t hg = u / p.passes, pass = u % p.passes;
-    const uint32_t h = blockIdx.y / p.pass_rows, r = blockIdx.y % p.pass_rows, gr_row = pass * p.pass_rows + r;
-    const uint32_t n_q = min(tokens_of(p, s), p.max_q);
-    if (gr_row >= n_q * p.group) return;
-    const uint64_t tok0 = p.cu_q ? p.cu_q[s] : (uint64_t)s * p.max_q;
-    const uint64_t head_row = (tok0 + gr_row / p.group) * p.n_head + (hg * p.kvb + h) * p.group + gr_row % p.group;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const uint32_t n = pages ? (uint32_t)(c1 - c0 + 1u) : 0u;
-    auto at = [&](uint32_t i) { return ((2ull * (c0 + i) + (i == 0 ? 1u : 0u)) * p.kvb + h) * p.pass_rows + r; };
+    const uint32_t before = p.prefix[s], all = p.prefix[s + 1] - before;
+    const uint32_t share = share_of(p.prefix[p.n_seqs], grid), unit = all / p.units_per_seq;
+    const uint32_t begin = before + u * unit + p.unit_cost;   // page 0
+    const uint32_t c0 = begin / share, c1 = all ? (begin + unit - p.unit_cost - 1u) / share : c0;
+    if (all && c0 == c1) return;
+    const uint32_t warp = W == 1 ? 0u : threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t hg = u / p.passes, pass = u % p.passes, row = blockIdx.y * ROWS + (W == 1 ? threadIdx.x >> 5 : 0u);
+    const uint32_t h = row / p.pass_rows, r = row % p.pass_rows, gr_row = pass * p.pass_rows + r;
+    if (row >= p.kvb * p.pass_rows || gr_row >= min(tokens_of(p, s), p.max_q) * p.group) return;   // whole warps; W > 1: the whole CTA
+    const uint32_t n = all ? c1 - c0 + 1u : 0u;
 
-    float m = NONE, wm = NONE, l = 0.f;
-    for (uint32_t i = lane; i < n; i += 32u) {
-        const float4 st = *reinterpret_cast<const float4 *>(p.ml + at(i) * 4u);
-        const float m_new = fmaxf(m, st.x);
-        l = l * brc::fast_exp2(m - m_new) + st.z * brc::fast_exp2(st.x - m_new);
-        m = m_new;
-        wm = fmaxf(wm, st.y);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
-        const float m_new = fmaxf(m, m2);
-        l = l * brc::fast_exp2(m - m_new) + l2 * brc::fast_exp2(m2 - m_new);
-        m = m_new;
-        wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-    }
-    float v[PER];
+    float m = NONE, wm = NONE, l = 0.f, v[PER];
 #pragma unroll
     for (uint32_t j = 0; j < PER; ++j) v[j] = 0.f;
-#pragma unroll 4
-    for (uint32_t i = warp; i < n; i += 8u) {
-        const float f = brc::fast_exp2(p.ml[at(i) * 4u + 1u] - wm);
-        const float *a = p.acc + at(i) * HD + lane * 4u;
+    for (uint32_t i0 = warp; i0 < n; i0 += B * W) {
+        float4 st[B], x[B][PER / 4];
+#pragma unroll
+        for (uint32_t q = 0; q < B; ++q) {
+            const uint32_t i = i0 + W * q;
+            st[q] = make_float4(NONE, NONE, 0.f, 0.f);
+#pragma unroll
+            for (uint32_t j = 0; j < PER / 4; ++j) x[q][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i < n) {
+                const uint64_t a = (uint64_t)((2u * (c0 + i) + (i == 0 ? 1u : 0u)) * p.kvb + h) * p.pass_rows + r;
+                st[q] = *reinterpret_cast<const float4 *>(p.ml + a * 4u);
+#pragma unroll
+                for (uint32_t j = 0; j < PER / 4; ++j) x[q][j] = *reinterpret_cast<const float4 *>(p.acc + a * HD + lane * 4u + 128u * j);
+            }
+        }
+        float m_new = m, w_new = wm;
+#pragma unroll
+        for (uint32_t q = 0; q < B; ++q) {
+            m_new = fmaxf(m_new, st[q].x);
+            w_new = fmaxf(w_new, st[q].y);
+        }
+        const float f = brc::fast_exp2(wm - w_new);
+        l *= brc::fast_exp2(m - m_new);
+#pragma unroll
+        for (uint32_t j = 0; j < PER; ++j) v[j] *= f;
+#pragma unroll
+        for (uint32_t q = 0; q < B; ++q) {
+            const float g = brc::fast_exp2(st[q].y - w_new);
+            l += st[q].z * brc::fast_exp2(st[q].x - m_new);
+#pragma unroll
+            for (uint32_t j = 0; j < PER / 4; ++j) {
+                v[4 * j] += x[q][j].x * g;
+                v[4 * j + 1] += x[q][j].y * g;
+                v[4 * j + 2] += x[q][j].z * g;
+                v[4 * j + 3] += x[q][j].w * g;
+            }
+        }
+        m = m_new;
+        wm = w_new;
+    }
+    const uint64_t tok0 = p.cu_q ? p.cu_q[s] : (uint64_t)s * p.max_q;
+    const uint64_t head_row = (tok0 + gr_row / p.group) * p.n_head + (hg * p.kvb + h) * p.group + gr_row % p.group;
+    if constexpr (W == 1) {
+        const float f = l == 0.f ? 0.f : brc::fast_exp2(wm - m - WEIGHT_SHIFT) / l;
 #pragma unroll
         for (uint32_t j = 0; j < PER; j += 4) {
-            const float4 x = *reinterpret_cast<const float4 *>(a + 32u * j);
-            v[j] += x.x * f;
-            v[j + 1] += x.y * f;
-            v[j + 2] += x.z * f;
-            v[j + 3] += x.w * f;
+            float x[4] = {v[j] * f, v[j + 1] * f, v[j + 2] * f, v[j + 3] * f};
+            finish_row(p, HD, head_row, lane * 4u + 32u * j, x);
         }
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < PER; j += 4) *reinterpret_cast<float4 *>(&part[warp][lane * 4u + 32u * j]) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        if (lane == 0) warp_stat[warp] = make_float4(m, wm, l, 0.f);
+        __syncthreads();
+        const uint32_t d = threadIdx.x * 4u;
+        if (d >= HD) return;
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        m = wm = NONE;
+        l = 0.f;
+#pragma unroll
+        for (uint32_t w = 0; w < W; ++w) {
+            m = fmaxf(m, warp_stat[w].x);
+            wm = fmaxf(wm, warp_stat[w].y);
+        }
+#pragma unroll
+        for (uint32_t w = 0; w < W; ++w) {
+            const float4 st = warp_stat[w];
+            const float g = brc::fast_exp2(st.y - wm);
+            l += st.z * brc::fast_exp2(st.x - m);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] += part[w][d + e] * g;
+        }
+        const float f = l == 0.f ? 0.f : brc::fast_exp2(wm - m - WEIGHT_SHIFT) / l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] *= f;
+        finish_row(p, HD, head_row, d, x);
     }
-#pragma unroll
-    for (uint32_t j = 0; j < PER; j += 4) *reinterpret_cast<float4 *>(&part[warp][lane * 4u + 32u * j]) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-    __syncthreads();
-    const uint32_t d = threadIdx.x * 4u;
-    if (d >= HD) return;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t w = 0; w < 8; ++w)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] += part[w][d + e];
-    const float f = l == 0.f ? 0.f : brc::fast_exp2(wm - m - 15.f) / l;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] *= f;
-    finish_row(p, HD, head_row, d, x);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -707,46 +821,65 @@ Shape shape_of(const brc_pool *pool, uint32_t n_seqs, uint32_t n_head, uint32_t 
     s.passes = (uint32_t)((rows + s.pass_rows - 1u) / s.pass_rows);
     s.units_per_seq = pool->n_kv_head / s.kvb * s.passes;
     const uint64_t slots = 2ull * (uint64_t)pool->sm_count * s.kvb * s.pass_rows;
-    s.prefix_bytes = (((uint64_t)n_seqs + 1u) * 8u + 255u) / 256u * 256u;
+    s.prefix_bytes = (((uint64_t)n_seqs + 1u) * 4u + 255u) / 256u * 256u;
     s.ml_bytes = slots * 16u;
     s.acc_bytes = slots * pool->head_dim * 4u;
     return s;
 }
 
-template <int HD, uint32_t CODE, bool PREC, int RT>
+template <int HD, uint32_t CODE, bool PREC, int RT, int W>
 brc_status launch(const brc_pool *pool, AttnParams p, uint32_t grid, uint32_t merge_rows, cudaStream_t st) {
-    auto kern = kv8_attn_kernel<HD, CODE, PREC, RT>;
-    const uint32_t turns = WARPS / (p.kvb * p.row_groups);
+    auto kern = kv8_attn_kernel<HD, CODE, PREC, RT, W>;
+    const uint32_t turns = W / (p.kvb * p.row_groups);
     // Ring depth: what fits, in multiples of the warps that take pages in turn, so that a stage is always consumed by the same
     // warps (a parity wait is only valid for a warp that knows the previous round of the barrier is over).
-    const Smem none = smem_layout(HD, p.kvb, p.pass_rows, PREC, 0);
-    p.n_stages = std::min((SMEM_LIMIT - none.total) / none.stage_bytes, MAX_STAGES) / turns * turns;
-    const uint32_t smem = smem_layout(HD, p.kvb, p.pass_rows, PREC, p.n_stages).total;
+    auto depth = [&](uint32_t q_bufs) {
+        uint32_t n = MAX_STAGES / turns * turns;
+        while (n > turns && smem_layout(HD, W, p.kvb, p.pass_rows, PREC, n, q_bufs).total > SMEM_LIMIT) n -= turns;
+        return n;
+    };
+    p.q_bufs = depth(2) == depth(1) ? 2u : 1u;   // the next unit's q is staged ahead where that costs no ring stage
+    p.n_stages = depth(p.q_bufs);
+    const uint32_t smem = smem_layout(HD, W, p.kvb, p.pass_rows, PREC, p.n_stages, p.q_bufs).total;
+    if (smem > SMEM_LIMIT) return brc_fail(BRC_ERR_UNSUPPORTED, "8-bit attention: %u bytes of shared memory", smem);
     static std::atomic<uint64_t> ready{0};   // devices on which this kernel may use all shared memory
     const uint64_t bit = 1ull << (pool->device & 63);
     if (!(ready.load(std::memory_order_relaxed) & bit) || pool->device > 63) {
         BRC_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_LIMIT));
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    kern<<<grid, THREADS, smem, st>>>(pool->tm_kv8, p);
-    BRC_CUDA(cudaGetLastError());
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.n_seqs * p.units_per_seq, merge_rows);
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
+    // Both kernels are launched so that they may come up while the one in front of them runs out (they wait for its end before they
+    // read anything).
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    BRC_CUDA(cudaLaunchKernelEx(&cfg, kv8_merge_kernel<HD>, p, grid));
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(W * 32 + 128);
+    cfg.dynamicSmemBytes = smem;
+    BRC_CUDA(cudaLaunchKernelEx(&cfg, kern, pool->tm_kv8, p));
+    cfg.dynamicSmemBytes = 0;
+    if ((uint64_t)p.n_seqs * p.units_per_seq * 4u <= grid) {
+        // Few units have many partials each (one long sequence: one from every SM): 16 warps a row fetch eighty at a time.
+        cfg.gridDim = dim3(p.n_seqs * p.units_per_seq, merge_rows);
+        cfg.blockDim = dim3(512);
+        BRC_CUDA(cudaLaunchKernelEx(&cfg, kv8_merge_kernel<HD, 16, 1, 5>, p, grid));
+    } else {   // many units have a few: a warp a row
+        cfg.gridDim = dim3(p.n_seqs * p.units_per_seq, (merge_rows + 7u) / 8u);
+        cfg.blockDim = dim3(256);
+        BRC_CUDA(cudaLaunchKernelEx(&cfg, kv8_merge_kernel<HD, 1, 8, 4>, p, grid));
+    }
     return BRC_OK;
 }
 
 template <int HD, uint32_t CODE>
 brc_status launch_rows(const brc_pool *pool, const AttnParams &p, uint32_t grid, bool prec, uint32_t rt, uint32_t merge_rows, cudaStream_t st) {
-    if (prec) return rt == 1 ? launch<HD, CODE, true, 1>(pool, p, grid, merge_rows, st) : launch<HD, CODE, true, 2>(pool, p, grid, merge_rows, st);
-    return rt == 1 ? launch<HD, CODE, false, 1>(pool, p, grid, merge_rows, st) : launch<HD, CODE, false, 2>(pool, p, grid, merge_rows, st);
+    constexpr int W1 = HD == 128 ? KV8_W1_128 : KV8_W1_256, W2 = HD == 128 ? KV8_W2_128 : KV8_W2_256;
+    if (prec) return rt == 1 ? launch<HD, CODE, true, 1, W1>(pool, p, grid, merge_rows, st) : launch<HD, CODE, true, 2, W2>(pool, p, grid, merge_rows, st);
+    return rt == 1 ? launch<HD, CODE, false, 1, W1>(pool, p, grid, merge_rows, st) : launch<HD, CODE, false, 2, W2>(pool, p, grid, merge_rows, st);
 }
 
 bool known_dtype(int32_t d) { return d == BRC_DTYPE_F32 || d == BRC_DTYPE_F16 || d == BRC_DTYPE_BF16; }
@@ -800,7 +933,7 @@ brc_status brc_kv8_attend(brc_pool *pool, const char *who, const brc_kv8_attn_ar
     p.k_layer = pool->k_base + (uint64_t)a.layer * pool->layer_bytes;
     p.v_layer = pool->v_base + (uint64_t)a.layer * pool->v_layer_bytes;
     uint8_t *ws = static_cast<uint8_t *>(a.workspace);
-    p.prefix = reinterpret_cast<uint64_t *>(ws);
+    p.prefix = reinterpret_cast<uint32_t *>(ws);
     p.ml = reinterpret_cast<float *>(ws + s.prefix_bytes);
     p.acc = reinterpret_cast<float *>(ws + s.prefix_bytes + s.ml_bytes);
     p.status = pool->status_dev;
@@ -823,7 +956,12 @@ brc_status brc_kv8_attend(brc_pool *pool, const char *who, const brc_kv8_attn_ar
     p.passes = s.passes;
     p.units_per_seq = s.units_per_seq;
     p.scale_log2 = a.scale * 1.4426950408889634f;
-    const uint64_t most = (uint64_t)a.n_seqs * s.units_per_seq * ((a.max_seq_len + 15ull) / 16u);   // page-units at most
+    // Starting and finishing a unit takes a CTA about as long as streaming UNIT_KIB.
+    p.unit_cost = std::max(1u, (UNIT_KIB * 1024u) / (s.kvb * 2u * 16u * pool->head_dim));
+    const uint64_t most = (uint64_t)a.n_seqs * s.units_per_seq * ((a.max_seq_len + 15ull) / 16u + p.unit_cost);   // cost at most
+    if (most >= (1ull << 31))
+        return brc_fail(BRC_ERR_UNSUPPORTED, "%s: %u sequences of up to %u cells in %u passes each are too much for one call", who, a.n_seqs, a.max_seq_len,
+                        s.units_per_seq);
     const uint32_t grid = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>(pool->sm_count, (most + MIN_SHARE - 1u) / MIN_SHARE));
     const bool prec = a.q_dtype == BRC_DTYPE_F32 || a.out_dtype == BRC_DTYPE_F32;
     const uint32_t merge_rows = s.kvb * s.pass_rows;
