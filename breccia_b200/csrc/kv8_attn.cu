@@ -93,7 +93,7 @@ __host__ __device__ inline Smem smem_layout(uint32_t hd, uint32_t warps, uint32_
     s.bars = at;                          // full, empty (ring); full, empty (q)
     at += 2u * MAX_STAGES * 8u + 32u;
     s.sched = at;
-    at += warps * 4u + 32u;
+    at += warps * 4u + 64u;
     s.total = at;
     return s;
 }
@@ -128,10 +128,13 @@ __device__ __forceinline__ void finish_row(const AttnParams &p, uint32_t hd, uin
     store_out(p, head_row * hd + d, v[0], v[1], v[2], v[3]);
 }
 
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-    return v;
+__device__ __forceinline__ uint4 lds128(const uint8_t *smem, uint32_t at) { return *reinterpret_cast<const uint4 *>(smem + at); }
+
+// D(16x8, f32) += A(16x16, f16, row) * B(16x8, f16, col).  Not volatile: the compiler may interleave it with the conversions.
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // One load of q rows in any of the three types: eight consecutive values of head row `r` from column d.
@@ -148,6 +151,11 @@ struct Cursor {
 
 struct Segment {
     uint32_t s, u, pg, n, pages;
+};
+
+struct Start {   // of a share: its first segment (n = 0: none) and where to go on
+    Cursor cur;
+    Segment seg;
 };
 
 __device__ __forceinline__ bool next_segment(const AttnParams &p, Cursor &c, Segment &g) {
@@ -233,21 +241,24 @@ __device__ __forceinline__ void stage_q(const AttnParams &p, const Smem &L, uint
     }
 }
 
-// RT: tiles of eight query rows that a warp carries; W: consuming warps.  PREC: q and the probabilities as two binary16 parts each.
-template <int HD, uint32_t CODE, bool PREC, int RT, int W>
+// RT: tiles of eight query rows that a warp carries; RG: warps side by side on a page's rows; KVB: kv heads of a unit; W: consuming
+// warps.  PREC: q and the probabilities as two binary16 parts each.
+template <int HD, uint32_t CODE, bool PREC, int RT, int RG, int KVB, int W>
 __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_constant__ CUtensorMap tm, const AttnParams p) {
     constexpr uint32_t SLABS = HD / 128, CONSUMERS = W * 32, ROW = HD + 4;
+    constexpr uint32_t STEP = KVB * RG, LANES = W / STEP, PASS = RG * RT * 8, STAGE = KVB * 2 * 16 * HD, SLAB = STAGE / SLABS;   // LANES: warps that take pages in turn
+    static_assert(W % STEP == 0 && CONSUMERS % (HD / 4) == 0, "");
     extern __shared__ __align__(1024) uint8_t smem[];
-    const Smem L = smem_layout(HD, W, p.kvb, p.pass_rows, PREC, p.n_stages, p.q_bufs);
+    const Smem L = smem_layout(HD, W, KVB, PASS, PREC, p.n_stages, p.q_bufs);
     const uint32_t base = brc::smem_u32(smem);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t full0 = base + L.bars, empty0 = full0 + MAX_STAGES * 8u, q_full0 = empty0 + MAX_STAGES * 8u, q_empty0 = q_full0 + 16u;
     uint32_t *warp_cost = reinterpret_cast<uint32_t *>(smem + L.sched);   // [W]: cost of each warp's sequences
-    Cursor *cursor = reinterpret_cast<Cursor *>(smem + L.sched + W * 4u);
+    Start *start = reinterpret_cast<Start *>(smem + L.sched + W * 4u);
     if (tid == CONSUMERS) {
         for (uint32_t i = 0; i < p.n_stages; ++i) {
             brc::mbar_init(full0 + 8u * i, 1u);
-            brc::mbar_init(empty0 + 8u * i, p.kvb * p.row_groups);       // the warps that read a stage
+            brc::mbar_init(empty0 + 8u * i, STEP);       // the warps that read a stage
         }
         for (uint32_t i = 0; i < p.q_bufs; ++i) {
             brc::mbar_init(q_full0 + 8u * i, 3u);                        // helper warps
@@ -300,7 +311,11 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
             }
             c /= p.units_per_seq;
             const uint32_t u = (lo - a) / c;
-            *cursor = Cursor{a + u * c, lo, hi, s, u};
+            Cursor first{a + u * c, lo, hi, s, u};
+            Segment seg = {};
+            seg.n = next_segment(p, first, seg) ? seg.n : 0u;
+            start->cur = first;
+            start->seg = seg;
         }
         if (blockIdx.x == 0) {   // for the merging kernel
             if (tid == 0) p.prefix[0] = 0;
@@ -314,8 +329,9 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
     }
     if (lo >= hi) return;
     __syncthreads();
-    Cursor cur = *cursor;
-    Segment g;
+    Cursor cur = start->cur;
+    Segment g = start->seg;
+    bool more = g.n != 0;
 
     // Registers: launched with 168 / 128 / 96 a thread (8 / 12 / 16 consuming warps and four more), of which the four others
     // keep 56 and hand the rest to the consumers; the sums stay within what the block was launched with.
@@ -325,7 +341,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
         if (warp > W) {
             // -------------------------------------------------------------- helpers: q of every unit but the first
             uint32_t idx = 0;
-            while (next_segment(p, cur, g)) {
+            for (; more; more = next_segment(p, cur, g)) {
                 if (idx) {
                     const uint32_t buf = idx % p.q_bufs;
                     if (idx >= p.q_bufs) ok = brc::mbar_wait(q_empty0 + 8u * buf, (idx - p.q_bufs) / p.q_bufs & 1u);
@@ -343,8 +359,8 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
             const uint64_t policy = brc::l2_policy_evict_first();
             const uint32_t j = lane / SLABS, sl = lane % SLABS;
             uint32_t stage = 0, parity = 1;   // the first round finds every stage empty
-            while (ok && next_segment(p, cur, g)) {
-                const uint32_t row0 = (g.u / p.passes) * p.kvb * 16u;
+            for (; ok && more; more = next_segment(p, cur, g)) {
+                const uint32_t row0 = (g.u / p.passes) * KVB * 16u;
                 const uint32_t *table = p.block_tables + (uint64_t)g.s * p.table_stride + g.pg;
                 uint32_t ahead = lane < g.n ? table[lane] : 0u;
                 for (uint32_t i0 = 0; ok && i0 < g.n; i0 += 32u) {
@@ -359,11 +375,11 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
                         const uint32_t st = wrap ? stage + j - p.n_stages : stage + j;
                         if (mine) {
                             ok = brc::mbar_wait(empty0 + 8u * st, wrap ? parity ^ 1u : parity);
-                            if (ok && sl == 0) brc::mbar_arrive_expect_tx(full0 + 8u * st, L.stage_bytes);
+                            if (ok && sl == 0) brc::mbar_arrive_expect_tx(full0 + 8u * st, STAGE);
                         }
                         ok = __all_sync(0xffffffffu, ok);
                         if (mine && ok)
-                            brc::tma_load_4d(base + st * L.stage_bytes + sl * (L.stage_bytes / SLABS), &tm, (int32_t)(sl * 128u), (int32_t)row0,
+                            brc::tma_load_4d(base + st * STAGE + sl * (SLAB), &tm, (int32_t)(sl * 128u), (int32_t)row0,
                                              (int32_t)(p.page0 + id), 0, full0 + 8u * st, policy);
                         stage += min(BATCH, m - i);
                         if (stage >= p.n_stages) { stage -= p.n_stages; parity ^= 1u; }
@@ -380,22 +396,19 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
 
     // ---------------------------------------------------------------------- consumers
     const uint32_t t = lane & 3u, gr = lane >> 2;            // thread of a group, group
-    const uint32_t hk = warp % p.kvb, rg = warp / p.kvb % p.row_groups;
-    const uint32_t lanes = W / (p.kvb * p.row_groups);   // warps that take pages in turn
-    const uint32_t pl = warp / (p.kvb * p.row_groups);
-    const uint32_t slab_bytes = p.kvb * 2u * 16u * 128u;     // [K|V][head][cell][128]
+    const uint32_t hk = warp % KVB, rg = warp / KVB % RG, pl = warp / STEP;
     float *scratch = reinterpret_cast<float *>(smem + L.scratch);
     float4 *stat = reinterpret_cast<float4 *>(smem + L.stat);
     const uint64_t code_bytes = (uint64_t)p.n_kv * 16u * HD;
     // Scales of this warp's next 32 page-units of a segment, one a lane, in two steps so that nobody waits for a page id:
     // ids_of asks for the ids, scales_of some time later for the scales.  An id out of range shows as a negative scale.
     auto ids_of = [&](const Segment &g, uint32_t i0) {
-        const uint32_t i = i0 + lanes * lane;
+        const uint32_t i = i0 + LANES * lane;
         return i < g.n ? p.block_tables[(uint64_t)g.s * p.table_stride + g.pg + i] : 0u;
     };
     auto scales_of = [&](const Segment &g, uint32_t id, float &ks, float &vs) {
         if (id < p.n_pages) {
-            const uint64_t at = id * p.page_bytes + code_bytes + (g.u / p.passes * p.kvb + hk) * 4u;
+            const uint64_t at = id * p.page_bytes + code_bytes + (g.u / p.passes * KVB + hk) * 4u;
             ks = *reinterpret_cast<const float *>(p.k_layer + at);
             vs = *reinterpret_cast<const float *>(p.v_layer + at);
         } else {
@@ -409,7 +422,6 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
     bool ok = true;
 
     Segment g_next;
-    bool more = next_segment(p, cur, g);
     uint32_t ids = more ? ids_of(g, pl) : 0u;
     while (more) {
         const uint32_t hg = g.u / p.passes, pass = g.u % p.passes;
@@ -429,10 +441,10 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
             scales_of(g, ids, ks_next, vs_next);
             ok = ok && brc::mbar_wait(q_full0 + 8u * buf_q, (idx - 1u) / p.q_bufs & 1u);
         }
-        const float *row_fac = reinterpret_cast<const float *>(smem + L.row_fac) + (buf_q * p.kvb + hk) * p.pass_rows;
-        const uint32_t *row_vis = reinterpret_cast<const uint32_t *>(smem + L.row_vis) + buf_q * p.pass_rows;
-        const uint32_t q_at = buf_q * L.q_bytes + (hk * p.pass_rows + rg * RT * 8u) * HD * 2u + lane * 16u;
-        const uint32_t q_frag = base + L.q + q_at, q_frag_lo = base + L.q_lo + q_at;
+        const float *row_fac = reinterpret_cast<const float *>(smem + L.row_fac) + (buf_q * KVB + hk) * PASS;
+        const uint32_t *row_vis = reinterpret_cast<const uint32_t *>(smem + L.row_vis) + buf_q * PASS;
+        const uint32_t q_at = buf_q * L.q_bytes + (hk * PASS + rg * RT * 8u) * HD * 2u + lane * 16u;
+        const uint32_t q_frag = L.q + q_at, q_frag_lo = L.q_lo + q_at;
 
         float o[RT][SLABS * 8][4];
         float m_run[RT][2], w_run[RT][2], l_run[RT][2], fac[RT][2];
@@ -453,18 +465,18 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
             }
         }
 
-        for (uint32_t i = (pl + lanes - done % lanes) % lanes, k = 0; i < g.n; i += lanes, ++k) {
+        for (uint32_t i = (pl + LANES - done % LANES) % LANES, k = 0; i < g.n; i += LANES, ++k) {
             if (k % 32u == 0u) {
                 ks_now = ks_next;
                 vs_now = vs_next;
-                ids = ids_of(g, i + lanes * 32u);
+                ids = ids_of(g, i + LANES * 32u);
             } else if (k % 32u == 16u) {
                 scales_of(g, ids, ks_next, vs_next);
             }
             const float ks = __shfl_sync(0xffffffffu, ks_now, k % 32u), vs = __shfl_sync(0xffffffffu, vs_now, k % 32u);
             ok = ok && brc::mbar_wait(full0 + 8u * stage, parity);
             if (!ok) break;   // the producer gave up or its copy never came: no further wait, the sums stay as they are
-            const uint32_t buf = base + stage * L.stage_bytes;
+            const uint32_t buf = stage * STAGE;
             const uint32_t cell0 = (g.pg + i) * 16u;
 
             // ---- S^T[16 cells][8 rows] = K q^T, over exact codes
@@ -479,7 +491,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
 #pragma unroll
                 for (uint32_t c = 0; c < SLABS * 2u; ++c) {   // 16-byte column groups of this thread
                     const uint32_t col = ((2u * t + (c & 1u)) ^ gr) * 16u;
-                    const uint4 a = lds128(k_row + (c >> 1) * slab_bytes + col), b = lds128(k_row + (c >> 1) * slab_bytes + col + 8u * 128u);
+                    const uint4 a = lds128(smem, k_row + (c >> 1) * SLAB + col), b = lds128(smem, k_row + (c >> 1) * SLAB + col + 8u * 128u);
                     const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
                     for (uint32_t x = 0; x < 4; x += 2) {
@@ -491,13 +503,13 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
                         const uint32_t at = (c * 2u + x / 2u) * 512u;
 #pragma unroll
                         for (int n = 0; n < RT; ++n) {
-                            const uint4 qf = lds128(q_frag + n * 8u * HD * 2u + at);
-                            brc::mma_16816(part[n][0], f0, qf.x, qf.y);
-                            brc::mma_16816(part[n][1], f1, qf.z, qf.w);
+                            const uint4 qf = lds128(smem, q_frag + n * 8u * HD * 2u + at);
+                            mma(part[n][0], f0, qf.x, qf.y);
+                            mma(part[n][1], f1, qf.z, qf.w);
                             if (PREC) {
-                                const uint4 ql = lds128(q_frag_lo + n * 8u * HD * 2u + at);
-                                brc::mma_16816(part[n][0], f0, ql.x, ql.y);
-                                brc::mma_16816(part[n][1], f1, ql.z, ql.w);
+                                const uint4 ql = lds128(smem, q_frag_lo + n * 8u * HD * 2u + at);
+                                mma(part[n][0], f0, ql.x, ql.y);
+                                mma(part[n][1], f1, ql.z, ql.w);
                             }
                         }
                     }
@@ -576,7 +588,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
 #pragma unroll
                 for (uint32_t x = 0; x < 4; ++x) {
                     const uint32_t c = 2u * t + (x & 1u) + 8u * (x >> 1);
-                    const uint4 v = lds128(buf + sl * slab_bytes + ((p.kvb + hk) * 16u + c) * 128u + ((gr ^ (c & 7u)) * 16u));
+                    const uint4 v = lds128(smem, buf + sl * SLAB + ((KVB + hk) * 16u + c) * 128u + ((gr ^ (c & 7u)) * 16u));
                     w[x][0] = v.x;
                     w[x][1] = v.y;
                     w[x][2] = v.z;
@@ -604,15 +616,15 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
                     for (uint32_t j = 0; j < 4; ++j)
 #pragma unroll
                         for (int n = 0; n < RT; ++n) {
-                            brc::mma_16816(o[n][sl * 8u + 4u * y + j], fa[j], pw[n][0], pw[n][1]);
-                            if (PREC) brc::mma_16816(o[n][sl * 8u + 4u * y + j], fa[j], pw_lo[n][0], pw_lo[n][1]);
+                            mma(o[n][sl * 8u + 4u * y + j], fa[j], pw[n][0], pw[n][1]);
+                            if (PREC) mma(o[n][sl * 8u + 4u * y + j], fa[j], pw_lo[n][0], pw_lo[n][1]);
                         }
                 }
             }
             __syncwarp();
             if (lane == 0) brc::mbar_arrive(empty0 + 8u * stage);
-            stage += lanes;
-            if (stage >= p.n_stages) { stage -= p.n_stages; parity ^= 1u; }   // (n_stages is a multiple of lanes)
+            stage += LANES;
+            if (stage >= p.n_stages) { stage -= p.n_stages; parity ^= 1u; }   // (n_stages is a multiple of LANES)
         }
         done += g.n;
         __syncwarp();
@@ -633,7 +645,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
         const bool whole = g.n == g.pages;
         const uint64_t slot = 2ull * blockIdx.x + (g.pg == 0 ? 1u : 0u);
         more = next_segment(p, cur, g_next);
-        if (more) ids = ids_of(g_next, (pl + lanes - done % lanes) % lanes);   // on their way while this unit is merged
+        if (more) ids = ids_of(g_next, (pl + LANES - done % LANES) % LANES);   // on their way while this unit is merged
 #pragma unroll
         for (int n = 0; n < RT; ++n) {
 #pragma unroll
@@ -650,41 +662,54 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
                         }
             brc::named_bar_sync(1, CONSUMERS);
             {
-                constexpr uint32_t C4 = HD / 4;
-                const uint32_t items = p.kvb * p.row_groups * 8u * C4;
-                for (uint32_t it = tid; it < items; it += CONSUMERS) {
-                    const uint32_t d = it % C4 * 4u, row8 = it / C4 % 8u, wg = it / (8u * C4);   // wg = head + kvb * row group
-                    const uint32_t r = ((wg / p.kvb) * RT + n) * 8u + row8, h = wg % p.kvb;
-                    const uint32_t gr_row = pass * p.pass_rows + r;
-                    if (gr_row >= rows) continue;
-                    float m = NONE, wm = NONE;
-                    for (uint32_t q = 0; q < lanes; ++q) {
-                        const float4 st = stat[(wg + q * p.kvb * p.row_groups) * 16u + n * 8u + row8];
-                        m = fmaxf(m, st.x);
-                        wm = fmaxf(wm, st.y);
-                    }
-                    float l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-                    for (uint32_t q = 0; q < lanes; ++q) {
-                        const uint32_t w = wg + q * p.kvb * p.row_groups;
-                        const float4 st = stat[w * 16u + n * 8u + row8];
-                        l += st.z * brc::fast_exp2(st.x - m);
-                        const float f = brc::fast_exp2(st.y - wm);
-                        const float4 x = *reinterpret_cast<const float4 *>(scratch + (w * 8u + row8) * ROW + d);
-                        v[0] += x.x * f;
-                        v[1] += x.y * f;
-                        v[2] += x.z * f;
-                        v[3] += x.w * f;
-                    }
-                    if (whole) {
-                        const float f = l == 0.f ? 0.f : brc::fast_exp2(wm - m - WEIGHT_SHIFT) / l;
+                constexpr uint32_t C4 = HD / 4, U = 4;   // U groups of four values a thread side by side
+                const uint32_t items = STEP * 8u * C4;
+                for (uint32_t it0 = tid; it0 < items; it0 += U * CONSUMERS) {
+                    float m[U], wm[U], l[U], v[U][4];
+                    uint32_t at[U];   // stat row of the first warp that holds the item; 0 stands in past the end
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] *= f;
-                        const uint32_t tok = gr_row / p.group, head = (hg * p.kvb + h) * p.group + gr_row % p.group;
-                        finish_row(p, HD, (tok0 + tok) * p.n_head + head, d, v);
-                    } else {
-                        const uint64_t at = slot * p.kvb * p.pass_rows + h * p.pass_rows + r;
-                        *reinterpret_cast<float4 *>(p.acc + at * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
-                        if (d == 0) *reinterpret_cast<float4 *>(p.ml + at * 4u) = make_float4(m, wm, l, 0.f);
+                    for (uint32_t k = 0; k < U; ++k) {
+                        const uint32_t it = it0 + k * CONSUMERS, wg = it / (8u * C4);   // head + kvb * row group
+                        at[k] = it < items ? wg * 16u + n * 8u + it / C4 % 8u : 0u;
+                        m[k] = wm[k] = NONE;
+                        l[k] = v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0.f;
+                    }
+                    for (uint32_t q = 0; q < LANES; ++q)
+#pragma unroll
+                        for (uint32_t k = 0; k < U; ++k) {
+                            const float4 st = stat[at[k] + q * STEP * 16u];
+                            m[k] = fmaxf(m[k], st.x);
+                            wm[k] = fmaxf(wm[k], st.y);
+                        }
+                    const uint32_t d = it0 % C4 * 4u;   // CONSUMERS is a multiple of C4
+                    for (uint32_t q = 0; q < LANES; ++q)
+#pragma unroll
+                        for (uint32_t k = 0; k < U; ++k) {
+                            const float4 st = stat[at[k] + q * STEP * 16u];
+                            const float4 x = *reinterpret_cast<const float4 *>(scratch + ((at[k] / 16u + q * STEP) * 8u + at[k] % 8u) * ROW + d);
+                            const float f = brc::fast_exp2(st.y - wm[k]);
+                            l[k] += st.z * brc::fast_exp2(st.x - m[k]);
+                            v[k][0] += x.x * f;
+                            v[k][1] += x.y * f;
+                            v[k][2] += x.z * f;
+                            v[k][3] += x.w * f;
+                        }
+#pragma unroll
+                    for (uint32_t k = 0; k < U; ++k) {
+                        const uint32_t wg = at[k] / 16u, r = ((wg / KVB) * RT + n) * 8u + at[k] % 8u, h = wg % KVB;
+                        const uint32_t gr_row = pass * PASS + r;
+                        if (it0 + k * CONSUMERS >= items || gr_row >= rows) continue;
+                        if (whole) {
+                            const float f = l[k] == 0.f ? 0.f : brc::fast_exp2(wm[k] - m[k] - WEIGHT_SHIFT) / l[k];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[k][e] *= f;
+                            const uint32_t tok = gr_row / p.group, head = (hg * KVB + h) * p.group + gr_row % p.group;
+                            finish_row(p, HD, (tok0 + tok) * p.n_head + head, d, v[k]);
+                        } else {
+                            const uint64_t to = slot * KVB * PASS + h * PASS + r;
+                            *reinterpret_cast<float4 *>(p.acc + to * HD + d) = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
+                            if (d == 0) *reinterpret_cast<float4 *>(p.ml + to * 4u) = make_float4(m[k], wm[k], l[k], 0.f);
+                        }
                     }
                 }
                 brc::named_bar_sync(1, CONSUMERS);
@@ -827,10 +852,10 @@ Shape shape_of(const brc_pool *pool, uint32_t n_seqs, uint32_t n_head, uint32_t 
     return s;
 }
 
-template <int HD, uint32_t CODE, bool PREC, int RT, int W>
+template <int HD, uint32_t CODE, bool PREC, int RT, int RG, int KVB, int W>
 brc_status launch(const brc_pool *pool, AttnParams p, uint32_t grid, uint32_t merge_rows, cudaStream_t st) {
-    auto kern = kv8_attn_kernel<HD, CODE, PREC, RT, W>;
-    const uint32_t turns = W / (p.kvb * p.row_groups);
+    auto kern = kv8_attn_kernel<HD, CODE, PREC, RT, RG, KVB, W>;
+    const uint32_t turns = W / (KVB * RG);
     // Ring depth: what fits, in multiples of the warps that take pages in turn, so that a stage is always consumed by the same
     // warps (a parity wait is only valid for a warp that knows the previous round of the barrier is over).
     auto depth = [&](uint32_t q_bufs) {
@@ -862,7 +887,7 @@ brc_status launch(const brc_pool *pool, AttnParams p, uint32_t grid, uint32_t me
     cfg.dynamicSmemBytes = smem;
     BRC_CUDA(cudaLaunchKernelEx(&cfg, kern, pool->tm_kv8, p));
     cfg.dynamicSmemBytes = 0;
-    if ((uint64_t)p.n_seqs * p.units_per_seq * 4u <= grid) {
+    if ((uint64_t)p.n_seqs * p.units_per_seq * 8u <= grid) {
         // Few units have many partials each (one long sequence: one from every SM): 16 warps a row fetch eighty at a time.
         cfg.gridDim = dim3(p.n_seqs * p.units_per_seq, merge_rows);
         cfg.blockDim = dim3(512);
@@ -870,16 +895,22 @@ brc_status launch(const brc_pool *pool, AttnParams p, uint32_t grid, uint32_t me
     } else {   // many units have a few: a warp a row
         cfg.gridDim = dim3(p.n_seqs * p.units_per_seq, (merge_rows + 7u) / 8u);
         cfg.blockDim = dim3(256);
-        BRC_CUDA(cudaLaunchKernelEx(&cfg, kv8_merge_kernel<HD, 1, 8, 4>, p, grid));
+        BRC_CUDA(cudaLaunchKernelEx(&cfg, kv8_merge_kernel<HD, 1, 8, 6>, p, grid));
     }
     return BRC_OK;
 }
 
-template <int HD, uint32_t CODE>
-brc_status launch_rows(const brc_pool *pool, const AttnParams &p, uint32_t grid, bool prec, uint32_t rt, uint32_t merge_rows, cudaStream_t st) {
+template <int HD, uint32_t CODE, bool PREC, int KVB>
+brc_status launch_rows(const brc_pool *pool, const AttnParams &p, uint32_t grid, uint32_t rt, uint32_t merge_rows, cudaStream_t st) {
     constexpr int W1 = HD == 128 ? KV8_W1_128 : KV8_W1_256, W2 = HD == 128 ? KV8_W2_128 : KV8_W2_256;
-    if (prec) return rt == 1 ? launch<HD, CODE, true, 1, W1>(pool, p, grid, merge_rows, st) : launch<HD, CODE, true, 2, W2>(pool, p, grid, merge_rows, st);
-    return rt == 1 ? launch<HD, CODE, false, 1, W1>(pool, p, grid, merge_rows, st) : launch<HD, CODE, false, 2, W2>(pool, p, grid, merge_rows, st);
+    if (rt == 1) return launch<HD, CODE, PREC, 1, 1, KVB, W1>(pool, p, grid, merge_rows, st);
+    return p.row_groups == 1 ? launch<HD, CODE, PREC, 2, 1, KVB, W2>(pool, p, grid, merge_rows, st) : launch<HD, CODE, PREC, 2, 2, KVB, W2>(pool, p, grid, merge_rows, st);
+}
+
+template <int HD, uint32_t CODE>
+brc_status launch_kind(const brc_pool *pool, const AttnParams &p, uint32_t grid, bool prec, uint32_t rt, uint32_t merge_rows, cudaStream_t st) {
+    if (p.kvb == 2) return prec ? launch_rows<HD, CODE, true, 2>(pool, p, grid, rt, merge_rows, st) : launch_rows<HD, CODE, false, 2>(pool, p, grid, rt, merge_rows, st);
+    return prec ? launch_rows<HD, CODE, true, 1>(pool, p, grid, rt, merge_rows, st) : launch_rows<HD, CODE, false, 1>(pool, p, grid, rt, merge_rows, st);
 }
 
 bool known_dtype(int32_t d) { return d == BRC_DTYPE_F32 || d == BRC_DTYPE_F16 || d == BRC_DTYPE_BF16; }
@@ -969,11 +1000,11 @@ brc_status brc_kv8_attend(brc_pool *pool, const char *who, const brc_kv8_attn_ar
     brc_stage_begin(pool, BRC_STAGE_ATTN_PARTIAL, st);
     brc_status rc;
     if (pool->head_dim == 256)
-        rc = pool->kv8 == brc::KV8_E4M3 ? launch_rows<256, brc::KV8_E4M3>(pool, p, grid, prec, s.rt, merge_rows, st)
-                                        : launch_rows<256, brc::KV8_INT8>(pool, p, grid, prec, s.rt, merge_rows, st);
+        rc = pool->kv8 == brc::KV8_E4M3 ? launch_kind<256, brc::KV8_E4M3>(pool, p, grid, prec, s.rt, merge_rows, st)
+                                        : launch_kind<256, brc::KV8_INT8>(pool, p, grid, prec, s.rt, merge_rows, st);
     else
-        rc = pool->kv8 == brc::KV8_E4M3 ? launch_rows<128, brc::KV8_E4M3>(pool, p, grid, prec, s.rt, merge_rows, st)
-                                        : launch_rows<128, brc::KV8_INT8>(pool, p, grid, prec, s.rt, merge_rows, st);
+        rc = pool->kv8 == brc::KV8_E4M3 ? launch_kind<128, brc::KV8_E4M3>(pool, p, grid, prec, s.rt, merge_rows, st)
+                                        : launch_kind<128, brc::KV8_INT8>(pool, p, grid, prec, s.rt, merge_rows, st);
     brc_stage_end(pool, BRC_STAGE_ATTN_PARTIAL, st);
     return rc;
 }
