@@ -481,17 +481,26 @@ class IndexerState:
 
 
 _DTYPES = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+_WORD_TYPES = (torch.int32, torch.uint32)
+
+
+def _raw_stream(stream, device: int) -> int:
+    """The stream a call goes to: the one given, else the current one of the pool's GPU (whichever GPU is current)."""
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
 
 
 def _dtype(t: torch.dtype, who: str) -> int:
-    if t not in _DTYPES:
+    code = _DTYPES.get(t)
+    if code is None:
         raise BrcError(_lib.ERR_INVALID, f"{who}: dtype {t} (float32, float16 or bfloat16)")
-    return _DTYPES[t]
+    return code
 
 
 def _token_rows(t: torch.Tensor, heads: int, head_dim: int, who: str) -> int:
     """Elements from one token's row [heads, head_dim] (or [heads * head_dim]) to the next; the row itself is contiguous."""
     row = heads * head_dim
+    if t.is_contiguous() and t.dim() == 3 and t.shape[1] == heads and t.shape[2] == head_dim:
+        return row
     ok = (t.dim() == 2 and t.shape[1] == row and t.stride(1) == 1) or \
          (t.dim() == 3 and t.shape[1:] == (heads, head_dim) and t.stride(2) == 1 and (heads == 1 or t.stride(1) == head_dim))
     if not ok:
@@ -499,13 +508,13 @@ def _token_rows(t: torch.Tensor, heads: int, head_dim: int, who: str) -> int:
     return t.stride(0) if t.shape[0] > 1 else row
 
 
-def _words(t: torch.Tensor, device: int, who: str, n: int | None = None) -> torch.Tensor:
-    """A contiguous array of 32-bit words on the pool's GPU (what positions, lengths, tables and prefixes are)."""
-    if t.dtype not in (torch.int32, torch.uint32) or not t.is_contiguous() or t.device.index != device or not t.is_cuda:
+def _words(t: torch.Tensor, device: int, who: str, n: int | None = None) -> int:
+    """The address of a contiguous array of 32-bit words on the pool's GPU (what positions, lengths, tables and prefixes are)."""
+    if t.dtype not in _WORD_TYPES or not t.is_contiguous() or t.get_device() != device:
         raise BrcError(_lib.ERR_INVALID, f"{who}: {t.dtype} {tuple(t.shape)} on {t.device}: contiguous 32-bit words on cuda:{device} wanted")
     if n is not None and t.numel() != n:
         raise BrcError(_lib.ERR_INVALID, f"{who}: {t.numel()} words, {n} wanted")
-    return t
+    return t.data_ptr()
 
 
 class Rope:
@@ -528,39 +537,36 @@ class Rope:
         _lib.call("brc_rope_freqs", C.byref(a), self.turns_host.ctypes.data_as(C.POINTER(C.c_uint64)), C.byref(f))
         self.factor, self.n_rot, self.layout, self.device = f.value, n_rot, _lib.ROPE_LAYOUTS[layout], device
         self.turns = torch.from_numpy(self.turns_host.view(np.int64)).to(f"cuda:{device}") if torch.cuda.is_available() else None
+        self._turns_ptr = self.turns.data_ptr() if self.turns is not None else None
+        self._call = _lib.load().brc_rope_apply
+
+    def _side(self, name: str, x: torch.Tensor, y: torch.Tensor | None, tokens: int, hd: int, dtype: torch.dtype):
+        if y is None:
+            y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        if x.dim() != 3 or x.shape[2] != hd or x.shape[0] != tokens or y.shape != x.shape or y.dtype != x.dtype or x.dtype != dtype:
+            raise BrcError(_lib.ERR_INVALID, f"Rope.apply: {name} {tuple(x.shape)} {x.dtype} -> {tuple(y.shape)} {y.dtype} beside {tokens} tokens of "
+                                             f"heads of {hd}, {dtype}")
+        if x.get_device() != self.device or y.get_device() != self.device:
+            raise BrcError(_lib.ERR_INVALID, f"Rope.apply: {name} on {x.device} -> {y.device}, the frequencies on cuda:{self.device}")
+        heads = x.shape[1]
+        return y, heads, _token_rows(x, heads, hd, "Rope.apply"), _token_rows(y, heads, hd, "Rope.apply")
 
     def apply(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, q_out: torch.Tensor | None = None,
               k_out: torch.Tensor | None = None, stream=None):
         """q [tokens, n_head, head_dim], k [tokens, n_kv, head_dim] or None, positions [tokens] int32 -> (q_out, k_out), new
         tensors unless given (q_out=q rotates in place).  Tokens may be strided (columns of one projection)."""
-        hd = q.shape[-1]
-        pair = []
-        for name, x, y in (("q", q, q_out), ("k", k, k_out)):
-            if x is None:
-                pair += [None, None, 0, 0, 0]
-                continue
-            if y is None:
-                y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            if x.dim() != 3 or x.shape[2] != hd or x.shape[0] != q.shape[0] or y.shape != x.shape or y.dtype != x.dtype or x.dtype != q.dtype:
-                raise BrcError(_lib.ERR_INVALID, f"Rope.apply: {name} {tuple(x.shape)} {x.dtype} -> {tuple(y.shape)} {y.dtype} beside q {tuple(q.shape)} {q.dtype}")
-            if not x.is_cuda or x.device.index != self.device or y.device != x.device:
-                raise BrcError(_lib.ERR_INVALID, f"Rope.apply: {name} on {x.device}, the frequencies on cuda:{self.device}")
-            pair += [x, y, x.shape[1], _token_rows(x, x.shape[1], hd, "Rope.apply"), _token_rows(y, x.shape[1], hd, "Rope.apply")]
-        _words(positions, self.device, "Rope.apply: positions", q.shape[0])
-        qi, qo, qh, qs, qos, ki, ko, kh, ks, kos = pair
-        _lib.call("brc_rope_apply", self.device, _ptr(qi), _ptr(qo), qh, qs, qos, _ptr(ki), _ptr(ko), kh, ks, kos, hd,
-                  _dtype(q.dtype, "Rope.apply"), _ptr(positions), q.shape[0], _ptr(self.turns), self.n_rot, self.layout, self.factor,
-                  _stream_ptr(stream))
+        tokens, hd, dtype = q.shape[0], q.shape[-1], q.dtype
+        qo, qh, qs, qos = self._side("q", q, q_out, tokens, hd, dtype)
+        if k is None:
+            ko, k_ptr, ko_ptr, kh, ks, kos = None, None, None, 0, 0, 0
+        else:
+            ko, kh, ks, kos = self._side("k", k, k_out, tokens, hd, dtype)
+            k_ptr, ko_ptr = k.data_ptr(), ko.data_ptr()
+        at = _words(positions, self.device, "Rope.apply: positions", tokens)
+        _lib.check(self._call(self.device, q.data_ptr(), qo.data_ptr(), qh, qs, qos, k_ptr, ko_ptr, kh, ks, kos, hd,
+                              _dtype(dtype, "Rope.apply"), at, tokens, self._turns_ptr, self.n_rot, self.layout, self.factor,
+                              _raw_stream(stream, self.device)))
         return qo, ko
-
-
-def _kv8_spans(who: str, pool: KvPool, block_tables: torch.Tensor, pos0: torch.Tensor, cu_tokens, tokens_per_seq: int):
-    n_seqs = block_tables.shape[0]
-    _words(block_tables, pool.device, f"{who}: block_tables")
-    _words(pos0, pool.device, f"{who}: pos0", n_seqs)
-    if cu_tokens is not None:
-        _words(cu_tokens, pool.device, f"{who}: cu_tokens", n_seqs + 1)
-    return n_seqs, block_tables.shape[1]
 
 
 def kv8_append(pool: KvPool, layer: int, k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor, pos0: torch.Tensor,
@@ -568,31 +574,40 @@ def kv8_append(pool: KvPool, layer: int, k: torch.Tensor, v: torch.Tensor, block
                stream=None) -> None:
     """The quantising write into an 8-bit pool (brc_kv8_append): k / v [total_tokens, n_kv, hd] (tokens may be strided) at cells
     pos0[s] .. of each sequence, tokens_per_seq each or ragged by cu_tokens [n_seqs + 1] int32; `rope` rotates K on the way."""
-    n_seqs, stride = _kv8_spans("kv8_append", pool, block_tables, pos0, cu_tokens, tokens_per_seq)
-    if k.dtype != v.dtype or k.shape[0] != v.shape[0] or not k.is_cuda or k.device.index != pool.device or v.device != k.device:
+    device, n_kv, hd = pool.device, pool.n_kv_head, pool.head_dim
+    n_seqs, stride = block_tables.shape
+    total = k.shape[0]
+    if k.dtype != v.dtype or total != v.shape[0] or k.get_device() != device or v.get_device() != device:
         raise BrcError(_lib.ERR_INVALID, f"kv8_append: k {tuple(k.shape)} {k.dtype} {k.device}, v {tuple(v.shape)} {v.dtype} {v.device}")
-    if rope is not None and rope.device != pool.device:
-        raise BrcError(_lib.ERR_INVALID, f"kv8_append: the frequencies lie on cuda:{rope.device}, the pool on cuda:{pool.device}")
-    _lib.call("brc_kv8_append", pool.handle, layer, _ptr(block_tables), stride, _ptr(pos0), n_seqs, tokens_per_seq, _ptr(cu_tokens),
-              k.shape[0], max_pos_end, _ptr(k), _token_rows(k, pool.n_kv_head, pool.head_dim, "kv8_append"), _ptr(v),
-              _token_rows(v, pool.n_kv_head, pool.head_dim, "kv8_append"), _dtype(k.dtype, "kv8_append"),
-              _ptr(rope.turns) if rope else None, rope.n_rot if rope else 0, rope.layout if rope else 0, rope.factor if rope else 1.0,
-              _stream_ptr(stream))
+    if rope is None:
+        turns, n_rot, layout, factor = None, 0, 0, 1.0
+    else:
+        if rope.device != device:
+            raise BrcError(_lib.ERR_INVALID, f"kv8_append: the frequencies lie on cuda:{rope.device}, the pool on cuda:{device}")
+        turns, n_rot, layout, factor = rope._turns_ptr, rope.n_rot, rope.layout, rope.factor
+    _lib.check(_lib.load().brc_kv8_append(
+        pool.handle, layer, _words(block_tables, device, "kv8_append: block_tables"), stride, _words(pos0, device, "kv8_append: pos0", n_seqs),
+        n_seqs, tokens_per_seq, None if cu_tokens is None else _words(cu_tokens, device, "kv8_append: cu_tokens", n_seqs + 1), total, max_pos_end,
+        k.data_ptr(), _token_rows(k, n_kv, hd, "kv8_append"), v.data_ptr(), _token_rows(v, n_kv, hd, "kv8_append"), _dtype(k.dtype, "kv8_append"),
+        turns, n_rot, layout, factor, _raw_stream(stream, device)))
 
 
 def kv8_read(pool: KvPool, layer: int, block_tables: torch.Tensor, pos0: torch.Tensor, max_pos_end: int, tokens_per_seq: int = 1,
              cu_tokens: torch.Tensor | None = None, total_tokens: int | None = None, dtype: torch.dtype = torch.float16,
              stream=None) -> tuple[torch.Tensor, torch.Tensor]:
     """Cells pos0[s] .. of each sequence of an 8-bit pool as values (brc_kv8_read) -> K, V [total_tokens, n_kv, hd]."""
-    n_seqs, stride = _kv8_spans("kv8_read", pool, block_tables, pos0, cu_tokens, tokens_per_seq)
+    device = pool.device
+    n_seqs, stride = block_tables.shape
     if total_tokens is None:
         if cu_tokens is not None:
             raise BrcError(_lib.ERR_INVALID, "kv8_read: total_tokens is needed beside cu_tokens")
         total_tokens = n_seqs * tokens_per_seq
-    out = torch.empty((2, total_tokens, pool.n_kv_head, pool.head_dim), dtype=dtype, device=block_tables.device)
-    k, v = out.unbind(0)
-    _lib.call("brc_kv8_read", pool.handle, layer, _ptr(block_tables), stride, _ptr(pos0), n_seqs, tokens_per_seq, _ptr(cu_tokens),
-              total_tokens, max_pos_end, _ptr(k), _ptr(v), _dtype(dtype, "kv8_read"), _stream_ptr(stream))
+    tables, at = _words(block_tables, device, "kv8_read: block_tables"), _words(pos0, device, "kv8_read: pos0", n_seqs)
+    cu = None if cu_tokens is None else _words(cu_tokens, device, "kv8_read: cu_tokens", n_seqs + 1)
+    code = _dtype(dtype, "kv8_read")
+    k, v = torch.empty((2, total_tokens, pool.n_kv_head, pool.head_dim), dtype=dtype, device=block_tables.device).unbind(0)
+    _lib.check(_lib.load().brc_kv8_read(pool.handle, layer, tables, stride, at, n_seqs, tokens_per_seq, cu, total_tokens, max_pos_end, k.data_ptr(),
+                                        v.data_ptr(), code, _raw_stream(stream, device)))
     return k, v
 
 
@@ -610,23 +625,29 @@ def kv8_attend(pool: KvPool, layer: int, q: torch.Tensor, block_tables: torch.Te
     """Attention over an 8-bit pool for the last T tokens of each sequence (brc_kv8_attn): q [tokens, n_head, hd], T = max_q, or
     ragged by cu_q [n_seqs + 1] int32 with T <= max_q; token i of T sees seq_lens[s] - (T - 1 - i) cells.  `workspace` from
     kv8_workspace; calls that may run at the same time need one each."""
-    n_seqs = block_tables.shape[0]
-    _words(block_tables, pool.device, "kv8_attend: block_tables")
-    _words(seq_lens, pool.device, "kv8_attend: seq_lens", n_seqs)
-    if cu_q is not None:
-        _words(cu_q, pool.device, "kv8_attend: cu_q", n_seqs + 1)
-    elif q.shape[0] != n_seqs * max_q:
-        raise BrcError(_lib.ERR_INVALID, f"kv8_attend: {q.shape[0]} rows of q for {n_seqs} sequences of {max_q} tokens")
-    if q.dim() != 3 or q.shape[2] != pool.head_dim or not q.is_contiguous() or not q.is_cuda or q.device.index != pool.device:
+    device = pool.device
+    n_seqs, stride = block_tables.shape
+    if q.dim() != 3 or q.shape[2] != pool.head_dim or not q.is_contiguous() or q.get_device() != device:
         raise BrcError(_lib.ERR_INVALID, f"kv8_attend: q {tuple(q.shape)} on {q.device}: contiguous [tokens, n_head, {pool.head_dim}] wanted")
+    tokens, n_head, hd = q.shape
+    if cu_q is not None:
+        cu = _words(cu_q, device, "kv8_attend: cu_q", n_seqs + 1)
+    elif tokens != n_seqs * max_q:
+        raise BrcError(_lib.ERR_INVALID, f"kv8_attend: {tokens} rows of q for {n_seqs} sequences of {max_q} tokens")
+    else:
+        cu = None
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
-    elif out.shape != q.shape or not out.is_contiguous() or out.device != q.device:
+        out = torch.empty_like(q) if out_dtype is None else torch.empty_like(q, dtype=out_dtype)
+    elif out.shape != q.shape or not out.is_contiguous() or out.get_device() != device:
         raise BrcError(_lib.ERR_INVALID, f"kv8_attend: out {tuple(out.shape)} on {out.device} beside q {tuple(q.shape)}")
-    _lib.call("brc_kv8_attn", pool.handle, layer, _ptr(q), _dtype(q.dtype, "kv8_attend"), q.shape[1], _ptr(gate), gate_head_stride,
-              _ptr(block_tables), block_tables.shape[1], _ptr(seq_lens), _ptr(cu_q), n_seqs, max_q, max_seq_len,
-              1.0 / math.sqrt(pool.head_dim) if scale is None else scale, _ptr(out), _dtype(out.dtype, "kv8_attend"), _ptr(workspace),
-              workspace.numel() * workspace.element_size(), _stream_ptr(stream))
+    if workspace.get_device() != device or (gate is not None and (gate.get_device() != device or gate.dtype != torch.float32)):
+        raise BrcError(_lib.ERR_INVALID, f"kv8_attend: workspace on {workspace.device}, gate {None if gate is None else (gate.dtype, gate.device)}: "
+                                         f"cuda:{device} and float32 wanted")
+    _lib.check(_lib.load().brc_kv8_attn(
+        pool.handle, layer, q.data_ptr(), _dtype(q.dtype, "kv8_attend"), n_head, None if gate is None else gate.data_ptr(), gate_head_stride,
+        _words(block_tables, device, "kv8_attend: block_tables"), stride, _words(seq_lens, device, "kv8_attend: seq_lens", n_seqs), cu, n_seqs, max_q,
+        max_seq_len, 1.0 / math.sqrt(hd) if scale is None else scale, out.data_ptr(), _dtype(out.dtype, "kv8_attend"), workspace.data_ptr(),
+        workspace.nbytes, _raw_stream(stream, device)))
     return out
 
 
