@@ -53,6 +53,23 @@ __device__ __forceinline__ uint32_t kv8_encode4(float a, float b, float c, float
     return q(a) | (q(b) << 8) | (q(c) << 16) | (q(d) << 24);
 }
 
+// The same for finite values whose magnitude the scale covers (none saturates): v * inv, inv = 2^-e.  int8: adding 1.5 * 2^23 to
+// the exact product rounds it to an integer, ties to even, whose low byte is the code (the conversion instruction runs at
+// a quarter of the rate).
+template <uint32_t CODE>
+__device__ __forceinline__ uint32_t kv8_encode4_finite(float a, float b, float c, float d, float inv) {
+    if (CODE == KV8_E4M3) {
+        uint32_t r;
+        asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\tmov.b32 %0, {l, h};\n\t}"
+            : "=r"(r) : "f"(a * inv), "f"(b * inv), "f"(c * inv), "f"(d * inv));
+        return r;
+    }
+    const float m = 12582912.f;
+    const uint32_t x = __float_as_uint(fmaf(a, inv, m)), y = __float_as_uint(fmaf(b, inv, m)), z = __float_as_uint(fmaf(c, inv, m)),
+                   w = __float_as_uint(fmaf(d, inv, m));
+    return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+}
+
 // The four codes of a word as two pairs of exact binary16 numbers (bytes 0,1 and bytes 2,3).  int8: a byte with its sign bit flipped, under
 // the exponent byte 0x64, is the binary16 number 1024 + 128 + code; subtracting 1152 is exact.
 template <uint32_t CODE>
@@ -125,6 +142,64 @@ __device__ __forceinline__ void load8(const typename elem<DT>::t *p, bool vec, f
     }
 }
 
+// Eight consecutive elements as they lie in memory: half the registers of their f32 values for the 16-bit types.
+template <int DT>
+struct raw8 {
+    static constexpr int WORDS = DT == 0 ? 8 : 4;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const typename elem<DT>::t *p, bool vec) {
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4) {
+                const uint4 u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint32_t *>(p) + i);
+                w[i] = u.x;
+                w[i + 1] = u.y;
+                w[i + 2] = u.z;
+                w[i + 3] = u.w;
+            }
+        } else if constexpr (DT == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(p[i]);
+        } else {
+            const uint16_t *u = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[i] = 0u;
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            if constexpr (DT == 0) {
+                v[i] = __uint_as_float(w[i]);
+            } else if constexpr (DT == 1) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            } else {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    }
+    // Largest magnitude so far, as bits: magnitudes order like unsigned integers, infinities above every finite one and NaN
+    // above them.  16-bit types keep two running maxima in one word.
+    __device__ __forceinline__ void top(uint32_t &m) const {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) m = DT == 0 ? max(m, w[i] & 0x7fffffffu) : __vmaxu2(m, w[i] & 0x7fff7fffu);
+    }
+    // `top`'s word as the bits of an f32
+    static __device__ __forceinline__ uint32_t top_f32(uint32_t m) {
+        if constexpr (DT == 0) return m;
+        const uint32_t h = max(m >> 16, m & 0xffffu);
+        if constexpr (DT == 2) return h << 16;
+        return h > 0x7c00u ? 0x7fffffffu : __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+    }
+};
+
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if constexpr (DT == 1) {
@@ -178,13 +253,19 @@ struct page_tile {
 __host__ __device__ inline uint64_t tile_slots(uint32_t total_tokens, uint32_t n_seqs) { return (uint64_t)total_tokens / 16u + 2ull * n_seqs; }
 
 // False: an idle slot.  Cells at or past max_pos_end are cut off (*cut reports the first such cell, else UINT32_MAX).
+// Whole warps call it: the search for the sequence takes 32 steps at a time, a lane each (one load in front of the
+// others for up to 32 sequences, two for up to 1024; one by one they would be five and ten).
 __device__ __forceinline__ bool find_tile(uint64_t slot, const uint32_t *cu, uint32_t tokens_per_seq, uint32_t total, uint32_t n_seqs,
                                           const uint32_t *pos0, uint32_t max_pos_end, page_tile &t, uint32_t *cut) {
     auto begin = [&](uint32_t s) { return cu ? (uint64_t)min(cu[s], total) : (uint64_t)s * tokens_per_seq; };
-    uint32_t lo = 0, hi = n_seqs;   // largest s whose slots begin at or before `slot`
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t lo = 0, hi = n_seqs;   // largest s in [lo, hi) whose slots begin at or before `slot`
     while (hi - lo > 1u) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if (begin(mid) / 16u + 2ull * mid <= slot) lo = mid; else hi = mid;
+        const uint32_t step = (hi - lo + 31u) / 32u, s = lo + lane * step;
+        const bool in = s < hi && begin(s) / 16u + 2ull * s <= slot;   // true for lane 0, and false from some lane on
+        const uint32_t last = (uint32_t)__popc(__ballot_sync(0xffffffffu, in)) - 1u;
+        lo += last * step;
+        hi = min(hi, lo + step);
     }
     const uint64_t b = begin(lo), e = begin(lo + 1u);
     *cut = UINT32_MAX;

@@ -1,11 +1,12 @@
 // The 8-bit cache as it is written and read back (value = code * 2^e, one exponent per page, kv head and side).
 //
 // brc_kv8_append: one CTA per (page touched, side, group of kv heads).  The page is the unit because the scale is:
-// its 128 threads hold the page's new rows in registers (16 x head_dim values, eight consecutive ones at a time), take
+// its 128 threads hold a head's new rows in registers (16 x head_dim values, eight consecutive ones at a time), take
 // their largest magnitude, and with it the exponent; a page that already holds cells of this sequence keeps the
 // larger of its own and the needed exponent, and only when it grows are the kept codes read and rounded again.  K may
-// be rotated on the way, so that neither the rotated rows nor a second launch go through memory.
-// Bound: HBM for chunks (source rows once, one byte per value written), the launch for a decode step.
+// be rotated on the way, so that neither the rotated rows nor a second launch go through memory; the cos / sin pairs of
+// the page's positions are computed once for all heads of the CTA.  While a head is encoded the next one's rows are on
+// their way.  Bound: HBM for chunks (source rows once, one byte per value written), the launch for a decode step.
 //
 // brc_kv8_read: the inverse, one CTA per (page, side); HBM.
 #include "brc_internal.h"
@@ -35,100 +36,146 @@ __device__ void report(uint32_t *status, uint32_t bit, uint32_t value) {
     status[1] = value;
 }
 
-// The tile and its page; false for an idle slot or a refused page (reported once, by the CTA `first`).
-__device__ __forceinline__ bool tile_page(const PagesParams &p, bool first, page_tile &t, uint32_t &page) {
+// The CTA's tile; false for an idle slot.  A cut-off position is reported once, by the CTA `first`.
+__device__ __forceinline__ bool tile_of(const PagesParams &p, bool first, page_tile &t) {
     uint32_t cut;
     const bool live = brc::find_tile(blockIdx.x, p.cu_tokens, p.tokens_per_seq, p.total_tokens, p.n_seqs, p.pos0, p.max_pos_end, t, &cut);
     if (cut != UINT32_MAX && first && threadIdx.x == 0) report(p.status, BRC_DEV_BAD_POS, cut);
-    if (!live) return false;
-    page = p.block_tables[(uint64_t)t.seq * p.table_stride + t.cell0 / 16u];
-    if (page < p.n_pages) return true;
-    if (first && threadIdx.x == 0) report(p.status, BRC_DEV_BAD_PAGE, page);
-    return false;
+    return live;
 }
 
+// The eight values from column d of one new K row, rotated.  `row`: the row in memory, for pairs that no shuffle reaches.
+template <int DT, int HD>
+__device__ __forceinline__ void rotate8(const PagesParams &p, const typename brc::elem<DT>::t *row, const float2 *cs, uint32_t d, bool live,
+                                        const brc::raw8<DT> &raw, float (&v)[8]) {
+    const uint32_t half = p.n_rot / 2u;
+    if (p.interleaved) {
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j += 2)
+            if (d + j < p.n_rot) {
+                const float2 a = cs[(d + j) / 2u];
+                const float x = v[j], y = v[j + 1];
+                v[j] = x * a.x - y * a.y;
+                v[j + 1] = x * a.y + y * a.x;
+            }
+    } else if (half % 8u == 0u) {   // a chunk lies in one half, its partners are the chunk half / 8 lanes away
+        const bool second = d >= half;
+        const uint32_t lane = threadIdx.x & 31u, from = d >= p.n_rot ? lane : second ? lane - half / 8u : lane + half / 8u;
+        brc::raw8<DT> other;
+#pragma unroll
+        for (int j = 0; j < brc::raw8<DT>::WORDS; ++j) other.w[j] = __shfl_sync(0xffffffffu, raw.w[j], from);
+        if (d < p.n_rot) {
+            float o[8];
+            other.values(o);
+            const float4 *a4 = reinterpret_cast<const float4 *>(cs + (second ? d - half : d));   // 16-byte aligned: d and half are multiples of 8
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j += 2) {
+                const float4 a = a4[j / 2u];
+                v[j] = second ? o[j] * a.y + v[j] * a.x : v[j] * a.x - o[j] * a.y;
+                v[j + 1] = second ? o[j + 1] * a.w + v[j + 1] * a.z : v[j + 1] * a.z - o[j + 1] * a.w;
+            }
+        }
+    } else if (live) {
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            const uint32_t e = d + j;
+            if (e >= p.n_rot) break;
+            const bool second = e >= half;
+            const float2 a = cs[second ? e - half : e];
+            const float o = brc::to_f32(row[second ? e - half : e + half]);
+            v[j] = second ? o * a.y + v[j] * a.x : v[j] * a.x - o * a.y;
+        }
+    }
+}
+
+// CTAs an SM that the compiler has to leave registers for: more of them hide the loads and barriers of one another until the
+// registers spill.  16 384 tokens, measured: 8 heads of 128, bf16, rotated 37.7 us at 8, 40.1 at 6, 42.9 at 5; 2 heads of 256, rotated
+// f16 25.7 at 5, 28.5 at 4, f32 29.7 at 4, 36.9 at 5.
+constexpr int append_ctas(int dt, int hd, bool rope) { return hd == 128 ? (rope ? (dt == 0 ? 6 : 8) : 9) : dt == 0 ? 4 : rope ? 5 : 6; }
+
 template <uint32_t CODE, int DT, int HD, bool ROPE>
-__global__ void __launch_bounds__(128) kv8_append_kernel(const PagesParams p) {
+__global__ void __launch_bounds__(128, append_ctas(DT, HD, ROPE)) kv8_append_kernel(const PagesParams p) {
     constexpr uint32_t CHUNKS = HD / 8, ROWS = 128 / CHUNKS, STEPS = 16 / ROWS;   // 8-value chunks of a row; rows at once; rounds
     using T = typename brc::elem<DT>::t;
-    extern __shared__ float2 cos_sin[];   // [16 cells][n_rot / 2] (ROPE, K only)
-    __shared__ float warp_max[2][4];
-    __shared__ int bad_any;
+    extern __shared__ __align__(16) float2 cos_sin[];   // [16 cells][n_rot / 2] (ROPE, K only)
+    __shared__ uint32_t warp_max[2][4];
     const bool is_v = blockIdx.y & 1u;
-    const uint32_t h0 = (blockIdx.y >> 1) * p.heads_per_cta;
+    const uint32_t h0 = (blockIdx.y >> 1) * p.heads_per_cta, h1 = min(h0 + p.heads_per_cta, p.n_kv_head);
     const uint32_t tid = threadIdx.x, chunk = tid % CHUNKS, row0 = tid / CHUNKS, d = chunk * 8u;
     page_tile t;
-    uint32_t page;
-    if (!tile_page(p, blockIdx.y == 0, t, page)) return;
-    const T *src = static_cast<const T *>(is_v ? p.v_src : p.k_src);
+    if (!tile_of(p, blockIdx.y == 0, t)) return;
+    const T *src = static_cast<const T *>(is_v ? p.v_src : p.k_src) + (uint64_t)t.token0 * (is_v ? p.v_stride : p.k_stride);
     const uint64_t stride = is_v ? p.v_stride : p.k_stride;
     const bool vec = is_v ? p.v_vec : p.k_vec;
+    const bool rotate = ROPE && !is_v;
+    brc::raw8<DT> next[STEPS];
+    auto load = [&](uint32_t h) {
+#pragma unroll
+        for (uint32_t i = 0; i < STEPS; ++i) {
+            const uint32_t r = row0 + i * ROWS;   // the r-th new row of the page
+            if (r < t.count) next[i].load(src + r * stride + (uint64_t)h * HD + d, vec);
+            else next[i].zero();
+        }
+    };
+    load(h0);   // the rows do not wait for the page's id
+    const uint32_t page = p.block_tables[(uint64_t)t.seq * p.table_stride + t.cell0 / 16u];
+    if (page >= p.n_pages) {
+        if (blockIdx.y == 0 && tid == 0) report(p.status, BRC_DEV_BAD_PAGE, page);
+        return;
+    }
     uint8_t *base = (is_v ? p.v_layer : p.k_layer) + (uint64_t)page * p.page_bytes;
     float *scales = reinterpret_cast<float *>(base + (uint64_t)p.n_kv_head * 16u * HD);
-    const bool rotate = ROPE && !is_v;
     const uint32_t half = p.n_rot / 2u;
-    if (tid == 0) bad_any = 0;
     if (rotate)
         for (uint32_t i = tid; i < t.count * half; i += 128u)
             cos_sin[i] = brc::rope_cos_sin(t.cell0 + t.first + i / half, p.turns[i % half], p.factor);
     __syncthreads();
-    bool bad = false;
-    for (uint32_t h = h0; h < min(h0 + p.heads_per_cta, p.n_kv_head); ++h) {
-        float v[STEPS][8];
-        float amax = 0.f;
+    for (uint32_t h = h0; h < h1; ++h) {
+        brc::raw8<DT> raw[STEPS];
+        float v[STEPS][8];   // rotated K alone; else the raw words are unpacked where they are encoded
+        uint32_t top = 0u;
 #pragma unroll
-        for (uint32_t i = 0; i < STEPS; ++i) {
-            const uint32_t r = row0 + i * ROWS;   // the r-th new row of the page
-            if (r >= t.count) continue;
-            const T *row = src + (uint64_t)(t.token0 + r) * stride + (uint64_t)h * HD;
-            brc::load8<DT>(row + d, vec, v[i]);
-            if (rotate && d < p.n_rot) {
-                const float2 *cs = cos_sin + r * half;
-                if (p.interleaved) {
+        for (uint32_t i = 0; i < STEPS; ++i) raw[i] = next[i];
+        if (h + 1u < h1) load(h + 1u);
+        if (rotate) {
 #pragma unroll
-                    for (uint32_t j = 0; j < 8; j += 2)
-                        if (d + j < p.n_rot) {
-                            const float2 a = cs[(d + j) / 2u];
-                            const float x = v[i][j], y = v[i][j + 1];
-                            v[i][j] = x * a.x - y * a.y;
-                            v[i][j + 1] = x * a.y + y * a.x;
-                        }
-                } else if (vec && half % 8u == 0u) {
-                    const bool second = d >= half;   // a chunk lies in one half: its partners are a chunk too
-                    float o[8];
-                    brc::load8<DT>(row + (second ? d - half : d + half), true, o);
+            for (uint32_t i = 0; i < STEPS; ++i) {
+                const uint32_t r = row0 + i * ROWS;
+                raw[i].values(v[i]);
+                rotate8<DT, HD>(p, src + r * stride + (uint64_t)h * HD, cos_sin + (r < t.count ? r : 0u) * half, d, r < t.count, raw[i], v[i]);
 #pragma unroll
-                    for (uint32_t j = 0; j < 8; ++j) {
-                        const float2 a = cs[second ? d + j - half : d + j];
-                        v[i][j] = second ? o[j] * a.y + v[i][j] * a.x : v[i][j] * a.x - o[j] * a.y;
-                    }
-                } else {
+                for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+            }
+        } else {
 #pragma unroll
-                    for (uint32_t j = 0; j < 8; ++j) {
-                        const uint32_t e = d + j;
-                        if (e >= p.n_rot) break;
-                        const bool second = e >= half;
-                        const float2 a = cs[second ? e - half : e];
-                        const float o = brc::to_f32(row[second ? e - half : e + half]);
-                        v[i][j] = second ? o * a.y + v[i][j] * a.x : v[i][j] * a.x - o * a.y;
-                    }
+            for (uint32_t i = 0; i < STEPS; ++i) raw[i].top(top);
+            top = brc::raw8<DT>::top_f32(top);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if ((tid & 31u) == 0u) warp_max[h & 1u][tid >> 5] = top;
+        const float old_scale = t.first ? scales[h] : 0.f;   // read by every thread in front of the barrier, written behind it
+        __syncthreads();                                     // two buffers: the next head's maxima cannot overtake this head's reads
+        top = max(max(warp_max[h & 1u][0], warp_max[h & 1u][1]), max(warp_max[h & 1u][2], warp_max[h & 1u][3]));
+        const bool bad = top >= 0x7f800000u;   // an infinity or NaN among them: the largest finite magnitude, once more and apart
+        if (bad) {
+            top = 0u;
+#pragma unroll
+            for (uint32_t i = 0; i < STEPS; ++i) {
+                if (!rotate) raw[i].values(v[i]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t a = __float_as_uint(v[i][j]) & 0x7fffffffu;
+                    if (a < 0x7f800000u) top = max(top, a);
                 }
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float a = fabsf(v[i][j]);
-                const bool finite = a <= 3.402823466e38f;   // infinities saturate and NaN becomes 0: neither sets the scale
-                bad |= !finite;
-                amax = fmaxf(amax, finite ? a : 0.f);
-            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            __syncthreads();
+            if ((tid & 31u) == 0u) warp_max[h & 1u][tid >> 5] = top;
+            __syncthreads();
+            top = max(max(warp_max[h & 1u][0], warp_max[h & 1u][1]), max(warp_max[h & 1u][2], warp_max[h & 1u][3]));
+            if (tid == 0) report(p.status, BRC_DEV_BAD_VALUE, t.token0);
         }
-#pragma unroll
-        for (int m = 16; m; m >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
-        if ((tid & 31u) == 0u) warp_max[h & 1u][tid >> 5] = amax;
-        const float old_scale = scales[h];   // read by every thread before the barrier, written behind it
-        __syncthreads();                     // two buffers: the next head's maxima cannot overtake this head's reads
-        amax = fmaxf(fmaxf(warp_max[h & 1u][0], warp_max[h & 1u][1]), fmaxf(warp_max[h & 1u][2], warp_max[h & 1u][3]));
-        int e = brc::kv8_exponent<CODE>(amax);
+        int e = brc::kv8_exponent<CODE>(__uint_as_float(top));
         uint8_t *codes = base + (uint64_t)h * 16u * HD;
         if (t.first) {
             const int e_old = brc::kv8_scale_exponent(old_scale);
@@ -151,56 +198,79 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(const PagesParams p) {
             e = max(e, e_old);
         }
         const float inv = brc::exp2_int(-e);
+        const bool plain = !bad && __uint_as_float(top) * inv <= (CODE == brc::KV8_E4M3 ? 448.f : 127.f);   // (the exponent's upper clamp may leave some to saturate)
 #pragma unroll
         for (uint32_t i = 0; i < STEPS; ++i) {
             const uint32_t r = row0 + i * ROWS;
             if (r >= t.count) continue;
-            *reinterpret_cast<uint2 *>(codes + (t.first + r) * HD + d) =
-                make_uint2(brc::kv8_encode4<CODE>(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv),
-                           brc::kv8_encode4<CODE>(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv));
+            if (!rotate) raw[i].values(v[i]);
+            uint2 w;
+            if (plain)
+                w = make_uint2(brc::kv8_encode4_finite<CODE>(v[i][0], v[i][1], v[i][2], v[i][3], inv),
+                               brc::kv8_encode4_finite<CODE>(v[i][4], v[i][5], v[i][6], v[i][7], inv));
+            else
+                w = make_uint2(brc::kv8_encode4<CODE>(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv),
+                               brc::kv8_encode4<CODE>(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv));
+            *reinterpret_cast<uint2 *>(codes + (t.first + r) * HD + d) = w;
         }
         if (tid == 0) scales[h] = brc::exp2_int(e);
     }
-    if (bad) bad_any = 1;
-    __syncthreads();
-    if (tid == 0 && bad_any) report(p.status, BRC_DEV_BAD_VALUE, t.token0);
 }
 
 template <uint32_t CODE, int DT, int HD>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const PagesParams p) {
-    constexpr uint32_t CHUNKS = HD / 8;
+    constexpr uint32_t N = DT == 0 ? 4 : 8, CHUNKS = HD / N, U = 4;   // a chunk: sixteen bytes of output; U of them in flight a thread
     using T = typename brc::elem<DT>::t;
     const bool is_v = blockIdx.y & 1u;
     page_tile t;
-    uint32_t page;
-    if (!tile_page(p, blockIdx.y == 0, t, page)) return;
+    if (!tile_of(p, blockIdx.y == 0, t)) return;
+    const uint32_t page = p.block_tables[(uint64_t)t.seq * p.table_stride + t.cell0 / 16u];
+    if (page >= p.n_pages) {
+        if (blockIdx.y == 0 && threadIdx.x == 0) report(p.status, BRC_DEV_BAD_PAGE, page);
+        return;
+    }
     const uint8_t *base = (is_v ? p.v_layer : p.k_layer) + (uint64_t)page * p.page_bytes;
     const float *scales = reinterpret_cast<const float *>(base + (uint64_t)p.n_kv_head * 16u * HD);
-    const uint64_t row = (uint64_t)p.n_kv_head * HD;
-    T *out = static_cast<T *>(is_v ? p.v_out : p.k_out) + t.token0 * row;
-    const uint32_t per_row = p.n_kv_head * CHUNKS, n = t.count * per_row;
-    constexpr uint32_t U = 4;
-    for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 256u * U) {   // U loads in flight a thread
-        uint2 w[U];
+    const uint32_t per_row = p.n_kv_head * CHUNKS, dr = 256u / per_row, dc = 256u % per_row;
+    T *out = static_cast<T *>(is_v ? p.v_out : p.k_out) + (uint64_t)t.token0 * per_row * N;
+    uint32_t r = threadIdx.x / per_row, c = threadIdx.x % per_row;
+    while (r < t.count) {
+        uint32_t w[U][N / 4];
         float s[U];
+        uint32_t at[U];
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t i = i0 + 256u * u;
-            if (i < n) {
-                const uint32_t r = i / per_row, c = i % per_row, h = c / CHUNKS;
-                w[u] = *reinterpret_cast<const uint2 *>(base + ((uint64_t)h * 16u + t.first + r) * HD + (c % CHUNKS) * 8u);
-                s[u] = scales[h];
+            at[u] = UINT32_MAX;
+            if (r < t.count) {
+                const uint32_t h = c / CHUNKS;
+                at[u] = r * per_row + c;
+                const uint8_t *from = base + (h * 16u + t.first + r) * HD + (c % CHUNKS) * N;
+                if constexpr (N == 8) {
+                    const uint2 x = __ldcs(reinterpret_cast<const uint2 *>(from));
+                    w[u][0] = x.x;
+                    w[u][1] = x.y;
+                } else {
+                    w[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(from));
+                }
+                s[u] = __ldg(scales + h);
             }
+            r += dr;
+            c += dc;
+            if (c >= per_row) { c -= per_row; ++r; }
         }
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t i = i0 + 256u * u;
-            if (i >= n) break;
-            float a[4], b[4];
-            brc::kv8_decode4_f32<CODE>(w[u].x, a);
-            brc::kv8_decode4_f32<CODE>(w[u].y, b);
-            const float v[8] = {a[0] * s[u], a[1] * s[u], a[2] * s[u], a[3] * s[u], b[0] * s[u], b[1] * s[u], b[2] * s[u], b[3] * s[u]};
-            brc::store8<DT>(out + (uint64_t)(i / per_row) * row + (i % per_row) * 8u, true, v);
+            if (at[u] == UINT32_MAX) break;
+            float v[N];
+#pragma unroll
+            for (uint32_t x = 0; x < N / 4; ++x) {
+                float a[4];
+                brc::kv8_decode4_f32<CODE>(w[u][x], a);
+#pragma unroll
+                for (uint32_t y = 0; y < 4; ++y) v[4 * x + y] = a[y] * s[u];
+            }
+            if constexpr (N == 8) brc::store8<DT>(out + (uint64_t)at[u] * N, true, v);
+            else *reinterpret_cast<float4 *>(out + (uint64_t)at[u] * N) = make_float4(v[0], v[1], v[2], v[3]);
         }
     }
 }
@@ -315,7 +385,9 @@ brc_status brc_kv8_append(brc_pool *pool, uint32_t layer, const uint32_t *block_
     p.k_vec = ((reinterpret_cast<uintptr_t>(k_src_dev) | (k_token_stride * size)) & 15u) == 0;
     p.v_vec = ((reinterpret_cast<uintptr_t>(v_src_dev) | (v_token_stride * size)) & 15u) == 0;
     const uint64_t tiles = brc::tile_slots(total_tokens, n_seqs);
-    p.heads_per_cta = 1;
+    // All heads of a page in one CTA once that still leaves every SM several (the search, the positions' cos and sin and the
+    // start are then paid once, and the next head's rows travel while one is encoded), one head a CTA for a decode step.
+    p.heads_per_cta = tiles * 2u >= 4ull * pool->sm_count ? pool->n_kv_head : 1u;
     const dim3 grid((uint32_t)tiles, 2u * ((pool->n_kv_head + p.heads_per_cta - 1u) / p.heads_per_cta));
     brc_stage_begin(pool, BRC_STAGE_KV_APPEND, brc_stream(stream));
     const cudaError_t e = BRC_KV8_DISPATCH(launch_append, pool, src_dtype, p, pool->head_dim, grid, brc_stream(stream));

@@ -4,10 +4,11 @@
 //   (x, y) -> factor * (x cos a - y sin a, x sin a + y cos a),   a = 2 pi * position * turns_j
 //
 // The angle is an integer product (kv8.cuh, rope_cos_sin): exact to position * 2^-65 turns at every position, without a
-// table (one of cos and sin for 10^6 positions of 128 pairs would be 1 GB).  A CTA computes the cos / sin pairs of its
-// tokens once, in shared memory, for all their heads, of q and k alike; then every thread moves 16-byte chunks, both
-// halves of a pair by the same thread, so a call may work in place.  Bound: HBM (each value read and written once);
-// the launch for a decode step.
+// table (one of cos and sin for 10^6 positions of 128 pairs would be 1 GB).  A warp takes a token: it computes the
+// cos / sin pairs of its position once, keeps those of its lanes' columns in registers, and goes over the token's
+// heads, of q and k alike, sixteen bytes a lane, the next rows on their way while one is turned.  A row is read whole
+// before it is written, so a call may work in place.  A pair's other half comes by shuffle where it lies whole chunks
+// away, else through shared memory.  Bound: HBM (each value read and written once); the launch for a decode step.
 #include <algorithm>
 #include <cmath>
 
@@ -20,99 +21,235 @@ struct RopeSide {
     const void *in;
     void *out;
     uint64_t in_stride, out_stride;   // elements from token to token
-    uint32_t heads, vec;              // vec: rows may be moved in 16-byte pieces
+    uint32_t heads;
 };
 
 struct RopeParams {
     RopeSide side[2];
     const uint32_t *positions;
     const uint64_t *turns;
-    uint32_t n_tokens, tokens_per_cta, head_dim, n_rot, interleaved;
+    uint32_t n_tokens, tokens_per_cta, splits, head_dim, n_rot, interleaved;
     float factor;
 };
 
-// Pairs [j, j + 8) of a head in the half layout, or values [d, d + 8) otherwise, eight at a time.
+// Sixteen bytes of a row in f32.
 template <int DT>
-__device__ __forceinline__ void rotate_side(const RopeParams &p, const RopeSide &s, const float2 *cos_sin, uint32_t tok0, uint32_t n_tok) {
-    using T = typename brc::elem<DT>::t;
-    const T *in = static_cast<const T *>(s.in);
-    T *out = static_cast<T *>(s.out);
-    const uint32_t half = p.n_rot / 2u, hd = p.head_dim;
-    const bool in_place = s.in == s.out && s.in_stride == s.out_stride;
-    if (s.vec) {
-        // items of a head: half layout: half / 8 chunk pairs then the untouched chunks; interleaved: all chunks
-        const uint32_t rot_items = p.interleaved ? p.n_rot / 8u : half / 8u;
-        const uint32_t items = rot_items + (in_place ? 0u : (hd - p.n_rot) / 8u);
-        const uint32_t per_tok = s.heads * items, n = n_tok * per_tok;
-        for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-            const uint32_t tk = i / per_tok, r = i % per_tok, h = r / items, c = r % items;
-            const T *x = in + (uint64_t)(tok0 + tk) * s.in_stride + (uint64_t)h * hd;
-            T *y = out + (uint64_t)(tok0 + tk) * s.out_stride + (uint64_t)h * hd;
-            const float2 *cs = cos_sin + tk * half;
-            float a[8];
-            if (c >= rot_items) {
-                const uint32_t d = p.n_rot + (c - rot_items) * 8u;
-                brc::load8<DT>(x + d, true, a);
-                brc::store8<DT>(y + d, true, a);
-            } else if (p.interleaved) {
-                const uint32_t d = c * 8u;
-                brc::load8<DT>(x + d, true, a);
-                float o[8];
+struct Chunk {
+    static constexpr int N = DT == 0 ? 4 : 8;
+    uint4 w;
+    __device__ __forceinline__ void values(float (&v)[N]) const {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (uint32_t j = 0; j < 8; j += 2) {
-                    const float2 w = cs[(d + j) / 2u];
-                    o[j] = a[j] * w.x - a[j + 1] * w.y;
-                    o[j + 1] = a[j] * w.y + a[j + 1] * w.x;
-                }
-                brc::store8<DT>(y + d, true, o);
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == 0) {
+                v[i] = __uint_as_float(u[i]);
+            } else if constexpr (DT == 1) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
             } else {
-                const uint32_t d = c * 8u;
-                float b[8], o[8], q[8];
-                brc::load8<DT>(x + d, true, a);
-                brc::load8<DT>(x + d + half, true, b);
-#pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) {
-                    const float2 w = cs[d + j];
-                    o[j] = a[j] * w.x - b[j] * w.y;
-                    q[j] = a[j] * w.y + b[j] * w.x;
-                }
-                brc::store8<DT>(y + d, true, o);
-                brc::store8<DT>(y + d + half, true, q);
+                v[2 * i] = __uint_as_float(u[i] << 16);
+                v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
             }
         }
-        return;
     }
-    const uint32_t items = half + (in_place ? 0u : hd - p.n_rot);   // pairs, then single untouched values
-    const uint32_t per_tok = s.heads * items;
-    const uint64_t n = (uint64_t)n_tok * per_tok;
-    for (uint64_t i = threadIdx.x; i < n; i += blockDim.x) {
-        const uint32_t tk = (uint32_t)(i / per_tok), r = (uint32_t)(i % per_tok), h = r / items, c = r % items;
-        const T *x = in + (uint64_t)(tok0 + tk) * s.in_stride + (uint64_t)h * hd;
-        T *y = out + (uint64_t)(tok0 + tk) * s.out_stride + (uint64_t)h * hd;
-        if (c >= half) {
-            const uint32_t d = p.n_rot + (c - half);
-            y[d] = x[d];
-            continue;
+    __device__ __forceinline__ void pack(const float (&v)[N]) {
+        if constexpr (DT == 0) w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        else w = make_uint4(brc::pack2<DT>(v[0], v[1]), brc::pack2<DT>(v[2], v[3]), brc::pack2<DT>(v[4], v[5]), brc::pack2<DT>(v[6], v[7]));
+    }
+};
+
+enum Pairing { INTERLEAVED, HALF_CHUNKS, HALF_ANY };   // HALF_CHUNKS: n_rot / 2 is whole chunks
+
+constexpr uint32_t ROPE_WARPS = 8, ROPE_MAX_PAIRS = 128, ROPE_STAGE = 256 + 8;   // staged values of a warp: 256, one word of shift every 32
+
+// Rows of HD values whose addresses are multiples of 16 bytes.  `splits` warps share a token's rows.  64 bytes a lane are turned
+// while the next 64 travel, three CTAs an SM: 16384 tokens of 40 x 128 bf16 in 55.1 us interleaved (6.1 TB/s), 56.6 half;
+// with 32 bytes a lane 58.0 and 59.7, with 16 and no look-ahead 58.3 and 74.9.
+template <int DT, int HD, int PAIR>
+__global__ void __launch_bounds__(ROPE_WARPS * 32, 3) rope_kernel(const RopeParams p) {
+    using T = typename brc::elem<DT>::t;
+    constexpr uint32_t N = Chunk<DT>::N, CHUNKS = HD / N, LPR = CHUNKS < 32 ? CHUNKS : 32, CPL = CHUNKS / LPR, RPW = 32 / LPR;   // lanes of a row, chunks of a lane, rows of a warp
+    __shared__ float2 pairs_all[ROPE_WARPS][ROPE_MAX_PAIRS];
+    __shared__ float stage_all[PAIR == HALF_ANY ? ROPE_WARPS : 1][PAIR == HALF_ANY ? ROPE_STAGE : 1];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, half = p.n_rot / 2u;
+    const uint32_t job = blockIdx.x * ROPE_WARPS + warp, tok = job / p.splits, split = job % p.splits;
+    if (tok >= p.n_tokens) return;
+    float2 *pairs = pairs_all[warp];
+    float *stage = stage_all[PAIR == HALF_ANY ? warp : 0];
+    const uint32_t heads_q = p.side[0].in ? p.side[0].heads : 0u, heads = heads_q + (p.side[1].in ? p.side[1].heads : 0u);
+    const uint32_t sub = lane / LPR, col = lane % LPR * N;
+    // this token's rows of each side (the side's fields picked by value: an indexed parameter would go through local memory)
+    const T *q_in = static_cast<const T *>(p.side[0].in) + (uint64_t)tok * p.side[0].in_stride;
+    const T *k_in = static_cast<const T *>(p.side[1].in) + (uint64_t)tok * p.side[1].in_stride;
+    T *q_out = static_cast<T *>(p.side[0].out) + (uint64_t)tok * p.side[0].out_stride, *k_out = static_cast<T *>(p.side[1].out) + (uint64_t)tok * p.side[1].out_stride;
+    uint32_t r = split * RPW + sub;
+    const uint32_t step = p.splits * RPW;
+    constexpr uint32_t F = 4 / CPL;   // rows of a lane in flight
+    Chunk<DT> next[F][CPL];
+    auto load = [&](uint32_t r) {
+#pragma unroll
+        for (uint32_t f = 0; f < F; ++f) {
+            const uint32_t rr = r + f * step;
+            if (rr >= heads) break;
+            const T *x = (rr < heads_q ? q_in + rr * HD : k_in + (rr - heads_q) * HD) + col;
+#pragma unroll
+            for (uint32_t k = 0; k < CPL; ++k) next[f][k].w = *reinterpret_cast<const uint4 *>(x + k * LPR * N);
         }
-        const uint32_t d0 = p.interleaved ? 2u * c : c, d1 = p.interleaved ? 2u * c + 1u : c + half;
-        const float a = brc::to_f32(x[d0]), b = brc::to_f32(x[d1]);
-        const float2 w = cos_sin[tk * half + c];
-        y[d0] = brc::from_f32<DT>(a * w.x - b * w.y);
-        y[d1] = brc::from_f32<DT>(a * w.y + b * w.x);
+    };
+    load(r);
+    const uint32_t pos = p.positions[tok];
+    for (uint32_t j = lane; j < half; j += 32u) pairs[j] = brc::rope_cos_sin(pos, p.turns[j], p.factor);
+    __syncwarp();
+    // cos and sin of the lane's columns (INTERLEAVED: of its pairs); the sine with the sign that a column's partner enters with
+    constexpr uint32_t CS = PAIR == INTERLEAVED ? N / 2 : N;
+    float c[CPL][CS], s[CPL][CS];
+#pragma unroll
+    for (uint32_t k = 0; k < CPL; ++k)
+#pragma unroll
+        for (uint32_t j = 0; j < CS; ++j) {
+            const uint32_t e = PAIR == INTERLEAVED ? (col + k * LPR * N) / 2u + j : col + k * LPR * N + j;
+            const bool in = e < (PAIR == INTERLEAVED ? half : p.n_rot);
+            const float2 w = pairs[!in ? 0u : PAIR == INTERLEAVED || e < half ? e : e - half];
+            c[k][j] = w.x;
+            s[k][j] = PAIR != INTERLEAVED && e < half ? -w.y : w.y;
+        }
+    for (uint32_t r0 = split * RPW; r0 < heads; r0 += F * step, r += F * step) {   // whole warps
+        Chunk<DT> rows[F][CPL];
+#pragma unroll
+        for (uint32_t f = 0; f < F; ++f)
+#pragma unroll
+            for (uint32_t k = 0; k < CPL; ++k) rows[f][k] = next[f][k];
+        if (r0 + F * step < heads) load(r + F * step);
+#pragma unroll
+        for (uint32_t f = 0; f < F; ++f) {
+            if (r0 + f * step >= heads) break;
+            const uint32_t rr = r + f * step;
+            const bool live = rr < heads;   // the lane's row exists
+            Chunk<DT>(&now)[CPL] = rows[f];
+            float v[CPL][N], o[CPL][N];
+#pragma unroll
+            for (uint32_t k = 0; k < CPL; ++k) now[k].values(v[k]);
+            if constexpr (PAIR == HALF_CHUNKS) {
+#pragma unroll
+                for (uint32_t k = 0; k < CPL; ++k) {
+                    const uint32_t d = col + k * LPR * N;
+                    const uint32_t q = d >= p.n_rot ? d / N : (d < half ? d + half : d - half) / N;   // the partner's chunk
+                    Chunk<DT> other;
+                    uint32_t u[4];
+                    const uint32_t from = sub * LPR + q % LPR;
+#pragma unroll
+                    for (uint32_t x = 0; x < 4; ++x) {
+                        u[x] = 0u;
+#pragma unroll
+                        for (uint32_t kk = 0; kk < CPL; ++kk) {
+                            const uint32_t w = __shfl_sync(0xffffffffu, x == 0 ? now[kk].w.x : x == 1 ? now[kk].w.y : x == 2 ? now[kk].w.z : now[kk].w.w, from);
+                            if (q / LPR == kk) u[x] = w;
+                        }
+                    }
+                    other.w = make_uint4(u[0], u[1], u[2], u[3]);
+                    other.values(o[k]);
+                }
+            } else if constexpr (PAIR == HALF_ANY) {
+                __syncwarp();
+#pragma unroll
+                for (uint32_t k = 0; k < CPL; ++k)
+#pragma unroll
+                    for (uint32_t j = 0; j < N; ++j) {
+                        const uint32_t i = sub * HD + col + k * LPR * N + j;
+                        stage[i + i / 32u] = v[k][j];
+                    }
+                __syncwarp();
+#pragma unroll
+                for (uint32_t k = 0; k < CPL; ++k)
+#pragma unroll
+                    for (uint32_t j = 0; j < N; ++j) {
+                        const uint32_t d = col + k * LPR * N + j, i = sub * HD + (d >= p.n_rot ? d : d < half ? d + half : d - half);
+                        o[k][j] = stage[i + i / 32u];
+                    }
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < CPL; ++k) {
+                float y[N];
+#pragma unroll
+                for (uint32_t j = 0; j < N; ++j) {
+                    const uint32_t d = col + k * LPR * N + j;
+                    if constexpr (PAIR == INTERLEAVED) {
+                        const float x = v[k][j], z = v[k][j ^ 1u], t = j & 1u ? x * c[k][j / 2] + z * s[k][j / 2] : x * c[k][j / 2] - z * s[k][j / 2];
+                        y[j] = d < p.n_rot ? t : x;
+                    } else {
+                        const float t = v[k][j] * c[k][j] + o[k][j] * s[k][j];
+                        y[j] = d < p.n_rot ? t : v[k][j];
+                    }
+                }
+                now[k].pack(y);
+                if (live) *reinterpret_cast<uint4 *>((rr < heads_q ? q_out + rr * HD : k_out + (rr - heads_q) * HD) + col + k * LPR * N) = now[k].w;
+            }
+        }
     }
 }
 
-// blockIdx.y = 0: q, 1: k (its own CTAs, so that a decode step's few tokens spread)
+// Any head size, any alignment: a pair, or an untouched value, a thread.
 template <int DT>
-__global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(256) rope_any_kernel(const RopeParams p) {
+    using T = typename brc::elem<DT>::t;
     extern __shared__ float2 cos_sin[];
     const uint32_t tok0 = blockIdx.x * p.tokens_per_cta;
-    const uint32_t n_tok = min(p.tokens_per_cta, p.n_tokens - tok0), half = p.n_rot / 2u;
+    const uint32_t n_tok = min(p.tokens_per_cta, p.n_tokens - tok0), half = p.n_rot / 2u, hd = p.head_dim;
     for (uint32_t i = threadIdx.x; i < n_tok * half; i += blockDim.x)
         cos_sin[i] = brc::rope_cos_sin(p.positions[tok0 + i / half], p.turns[i % half], p.factor);
     __syncthreads();
-    for (uint32_t s = 0; s < 2; ++s)
-        if (p.side[s].in) rotate_side<DT>(p, p.side[s], cos_sin, tok0, n_tok);
+    const uint32_t items = half + (hd - p.n_rot);   // pairs, then single untouched values
+    for (uint32_t side = 0; side < 2; ++side) {
+        const RopeSide &s = p.side[side];
+        if (!s.in) continue;
+        const uint32_t per_tok = s.heads * items;
+        const uint64_t n = (uint64_t)n_tok * per_tok;
+        for (uint64_t i = threadIdx.x; i < n; i += blockDim.x) {
+            const uint32_t tk = (uint32_t)(i / per_tok), r = (uint32_t)(i % per_tok), h = r / items, c = r % items;
+            const T *x = static_cast<const T *>(s.in) + (uint64_t)(tok0 + tk) * s.in_stride + (uint64_t)h * hd;
+            T *y = static_cast<T *>(s.out) + (uint64_t)(tok0 + tk) * s.out_stride + (uint64_t)h * hd;
+            if (c >= half) {
+                const uint32_t d = p.n_rot + (c - half);
+                y[d] = x[d];
+                continue;
+            }
+            const uint32_t d0 = p.interleaved ? 2u * c : c, d1 = p.interleaved ? 2u * c + 1u : c + half;
+            const float a = brc::to_f32(x[d0]), b = brc::to_f32(x[d1]);
+            const float2 w = cos_sin[tk * half + c];
+            y[d0] = brc::from_f32<DT>(a * w.x - b * w.y);
+            y[d1] = brc::from_f32<DT>(a * w.y + b * w.x);
+        }
+    }
+}
+
+template <int DT, int HD>
+void launch_rows(const RopeParams &p, uint32_t grid, cudaStream_t st) {
+    if (p.interleaved) rope_kernel<DT, HD, INTERLEAVED><<<grid, ROPE_WARPS * 32, 0, st>>>(p);
+    else if (p.n_rot / 2u % Chunk<DT>::N == 0) rope_kernel<DT, HD, HALF_CHUNKS><<<grid, ROPE_WARPS * 32, 0, st>>>(p);
+    else rope_kernel<DT, HD, HALF_ANY><<<grid, ROPE_WARPS * 32, 0, st>>>(p);
+}
+
+template <int DT>
+void launch(RopeParams &p, bool rows, uint32_t total_heads, int sm_count, cudaStream_t st) {
+    if (rows) {
+        // A warp a token; its rows over several warps while that leaves SMs short of them.
+        const uint32_t rpw = std::max(1u, 32u * Chunk<DT>::N / p.head_dim), most = (total_heads + rpw - 1u) / rpw;
+        const uint64_t want = 16ull * sm_count;
+        p.splits = (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(1u, want / p.n_tokens));
+        const uint64_t jobs = (uint64_t)p.n_tokens * p.splits;
+        const uint32_t grid = (uint32_t)((jobs + ROPE_WARPS - 1u) / ROPE_WARPS);
+        if (p.head_dim == 64) launch_rows<DT, 64>(p, grid, st);
+        else if (p.head_dim == 128) launch_rows<DT, 128>(p, grid, st);
+        else launch_rows<DT, 256>(p, grid, st);
+        return;
+    }
+    // Tokens per CTA: about 32 KiB of rows, fewer while that leaves SMs without a CTA, never more cos / sin pairs than 32 KiB.
+    const uint32_t bytes = total_heads * p.head_dim * brc::elem<DT>::size;
+    p.tokens_per_cta = std::min(std::max(1u, 32768u / bytes), std::max(1u, 8192u / p.n_rot));
+    p.tokens_per_cta = std::min(p.tokens_per_cta, std::max(1u, p.n_tokens / 296u));
+    const uint32_t smem = p.tokens_per_cta * (p.n_rot / 2u) * (uint32_t)sizeof(float2);
+    rope_any_kernel<DT><<<(p.n_tokens + p.tokens_per_cta - 1u) / p.tokens_per_cta, 256, smem, st>>>(p);
 }
 
 }  // namespace
@@ -181,6 +318,7 @@ brc_status brc_rope_apply(int32_t device, const void *q_dev, void *q_out_dev, ui
     const uint32_t heads[2] = {n_head, n_kv_head};
     const uint64_t is[2] = {q_token_stride, k_token_stride}, os[2] = {q_out_token_stride, k_out_token_stride};
     uint32_t total_heads = 0;
+    bool rows = head_dim == 64 || head_dim == 128 || head_dim == 256;   // the kernel of whole rows: these sizes, 16-byte aligned
     for (int s = 0; s < 2; ++s) {
         if (!in[s]) continue;
         const uint64_t row = (uint64_t)heads[s] * head_dim;
@@ -204,9 +342,7 @@ brc_status brc_rope_apply(int32_t device, const void *q_dev, void *q_out_dev, ui
             if (a0 < b1 && b0 < a1 && !(a0 == b0 && r.in_stride == r.out_stride))
                 return brc_fail(BRC_ERR_INVALID, "%s: %s and its output overlap without being the same rows", who, s ? "k" : "q");
         }
-        // 16-byte pieces: aligned rows, and pairs whose chunks of eight do not straddle the rotated part's edges
-        r.vec = ((at | (r.in_stride * size) | (r.out_stride * size)) & 15u) == 0 && head_dim % 8u == 0 && n_rot % 8u == 0 &&
-                (layout == BRC_ROPE_INTERLEAVED || (n_rot / 2u) % 8u == 0);
+        rows = rows && ((at | (r.in_stride * size) | (r.out_stride * size)) & 15u) == 0;
         total_heads += heads[s];
     }
     if (n_tokens == 0) return BRC_OK;
@@ -220,17 +356,12 @@ brc_status brc_rope_apply(int32_t device, const void *q_dev, void *q_out_dev, ui
     p.n_rot = n_rot;
     p.interleaved = layout == BRC_ROPE_INTERLEAVED;
     p.factor = factor;
-    // Tokens per CTA: about 32 KiB of rows (a few hundred chunks a thread's loop can overlap), fewer while that leaves
-    // SMs without a CTA, never more cos / sin pairs than 32 KiB of shared memory.
-    const uint32_t bytes = total_heads * head_dim * size;
-    p.tokens_per_cta = std::min(std::max(1u, 32768u / bytes), std::max(1u, 8192u / n_rot));
-    p.tokens_per_cta = std::min(p.tokens_per_cta, std::max(1u, n_tokens / 296u));
-    const uint32_t smem = p.tokens_per_cta * (n_rot / 2u) * (uint32_t)sizeof(float2);
-    const uint32_t grid = (n_tokens + p.tokens_per_cta - 1u) / p.tokens_per_cta;
+    int sm_count = 0;
+    BRC_CUDA(cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, device));
     cudaStream_t st = brc_stream(stream);
-    if (dtype == BRC_DTYPE_F32) rope_kernel<0><<<grid, 256, smem, st>>>(p);
-    else if (dtype == BRC_DTYPE_F16) rope_kernel<1><<<grid, 256, smem, st>>>(p);
-    else rope_kernel<2><<<grid, 256, smem, st>>>(p);
+    if (dtype == BRC_DTYPE_F32) launch<0>(p, rows, total_heads, sm_count, st);
+    else if (dtype == BRC_DTYPE_F16) launch<1>(p, rows, total_heads, sm_count, st);
+    else launch<2>(p, rows, total_heads, sm_count, st);
     BRC_CUDA(cudaGetLastError());
     return BRC_OK;
 }
