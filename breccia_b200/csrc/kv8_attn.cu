@@ -137,6 +137,9 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Keeps a rare case a branch: selects in its place would be paid by every page (40 of them at 256 columns).
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
+
 // One load of q rows in any of the three types: eight consecutive values of head row `r` from column d.
 __device__ __forceinline__ void load_q8(const AttnParams &p, uint64_t at, float (&v)[8]) {
     if (p.q_dtype == 0) brc::load8<0>(static_cast<const float *>(p.q) + at, true, v);
@@ -406,13 +409,14 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
         const uint32_t i = i0 + LANES * lane;
         return i < g.n ? p.block_tables[(uint64_t)g.s * p.table_stride + g.pg + i] : 0u;
     };
-    auto scales_of = [&](const Segment &g, uint32_t id, float &ks, float &vs) {
+    auto scales_of = [&](const Segment &g, uint32_t id, float &ks, float &ev) {
         if (id < p.n_pages) {
             const uint64_t at = id * p.page_bytes + code_bytes + (g.u / p.passes * KVB + hk) * 4u;
             ks = *reinterpret_cast<const float *>(p.k_layer + at);
-            vs = *reinterpret_cast<const float *>(p.v_layer + at);
+            ev = (float)brc::kv8_scale_exponent(*reinterpret_cast<const float *>(p.v_layer + at));
         } else {
-            ks = vs = -1.f;
+            ks = -1.f;
+            ev = 0.f;
             atomicOr(p.status, BRC_DEV_BAD_PAGE);
             p.status[1] = id;
         }
@@ -430,15 +434,15 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
         const uint32_t rows = min(n_q, p.max_q) * p.group;               // of a kv head, over all passes
         const uint32_t vis_min = len + 1u > n_q ? len + 1u - n_q : 0u;   // cells that every row sees
         const uint32_t buf_q = idx % p.q_bufs;
-        float ks_now = 1.f, vs_now = 1.f, ks_next = 1.f, vs_next = 1.f;
+        float ks_now = 1.f, ev_now = 0.f, ks_next = 1.f, ev_next = 0.f;
         if (idx == 0) {   // the first unit's q: nobody has anything else to do yet
             // (scales asked for with the q rows: behind the first pages' boxes they would come 3 us later)
             bool asked = false;
-            stage_q<HD, PREC, 2>(p, L, smem, g, 0, warp, W, lane, [&] { scales_of(g, ids, ks_next, vs_next); asked = true; });
-            if (!asked) scales_of(g, ids, ks_next, vs_next);
+            stage_q<HD, PREC, 2>(p, L, smem, g, 0, warp, W, lane, [&] { scales_of(g, ids, ks_next, ev_next); asked = true; });
+            if (!asked) scales_of(g, ids, ks_next, ev_next);
             brc::named_bar_sync(1, CONSUMERS);
         } else {
-            scales_of(g, ids, ks_next, vs_next);
+            scales_of(g, ids, ks_next, ev_next);
             ok = ok && brc::mbar_wait(q_full0 + 8u * buf_q, (idx - 1u) / p.q_bufs & 1u);
         }
         const float *row_fac = reinterpret_cast<const float *>(smem + L.row_fac) + (buf_q * KVB + hk) * PASS;
@@ -468,12 +472,12 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
         for (uint32_t i = (pl + LANES - done % LANES) % LANES, k = 0; i < g.n; i += LANES, ++k) {
             if (k % 32u == 0u) {
                 ks_now = ks_next;
-                vs_now = vs_next;
+                ev_now = ev_next;
                 ids = ids_of(g, i + LANES * 32u);
             } else if (k % 32u == 16u) {
-                scales_of(g, ids, ks_next, vs_next);
+                scales_of(g, ids, ks_next, ev_next);
             }
-            const float ks = __shfl_sync(0xffffffffu, ks_now, k % 32u), vs = __shfl_sync(0xffffffffu, vs_now, k % 32u);
+            const float ks = __shfl_sync(0xffffffffu, ks_now, k % 32u), ev = __shfl_sync(0xffffffffu, ev_now, k % 32u);
             ok = ok && brc::mbar_wait(full0 + 8u * stage, parity);
             if (!ok) break;   // the producer gave up or its copy never came: no further wait, the sums stay as they are
             const uint32_t buf = stage * STAGE;
@@ -523,7 +527,6 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
             // ---- softmax against the rows' reference exponents; weights to B fragments [cells][rows].  The references
             // move only when a score passes one by more than 2^HEADROOM, so an ordinary page needs no maximum across the warp.
             const bool good = ks > 0.f;
-            const float ev = (float)brc::kv8_scale_exponent(vs);
             const bool edge = cell0 + 16u > vis_min || !good;
             uint32_t pw[RT][2], pw_lo[RT][2];
 #pragma unroll
@@ -536,6 +539,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
                     s[n][x] *= kf;
                     s[n][x + 2] *= kf;
                     if (edge) {
+                        keep_branch();
                         if (!good || cell0 + gr >= vis[n][x]) s[n][x] = -INFINITY;
                         if (!good || cell0 + gr + 8u >= vis[n][x]) s[n][x + 2] = -INFINITY;
                     }
@@ -593,7 +597,12 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
                     w[x][1] = v.y;
                     w[x][2] = v.z;
                     w[x][3] = v.w;
-                    if (tail && (!good || cell0 + c >= len)) w[x][0] = w[x][1] = w[x][2] = w[x][3] = 0u;
+                }
+                if (tail) {
+                    keep_branch();
+#pragma unroll
+                    for (uint32_t x = 0; x < 4; ++x)
+                        if (!good || cell0 + 2u * t + (x & 1u) + 8u * (x >> 1) >= len) w[x][0] = w[x][1] = w[x][2] = w[x][3] = 0u;
                 }
 #pragma unroll
                 for (uint32_t y = 0; y < 2; ++y) {   // columns 4 y .. 4 y + 3 and those + 8
