@@ -189,7 +189,10 @@ struct raw8 {
     // above them.  16-bit types keep two running maxima in one word.
     __device__ __forceinline__ void top(uint32_t &m) const {
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) m = DT == 0 ? max(m, w[i] & 0x7fffffffu) : __vmaxu2(m, w[i] & 0x7fff7fffu);
+        for (int i = 0; i < WORDS; ++i) {
+            if constexpr (DT == 0) m = max(m, w[i] & 0x7fffffffu);
+            else asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7fff7fffu));
+        }
     }
     // `top`'s word as the bits of an f32
     static __device__ __forceinline__ uint32_t top_f32(uint32_t m) {
