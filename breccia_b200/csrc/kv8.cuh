@@ -265,14 +265,14 @@ __device__ __forceinline__ bool find_tile(uint64_t slot, const uint32_t *cu, uin
     uint32_t lo = 0, hi = n_seqs;   // largest s in [lo, hi) whose slots begin at or before `slot`
     while (hi - lo > 1u) {
         const uint32_t step = (hi - lo + 31u) / 32u, s = lo + lane * step;
-        const bool in = s < hi && begin(s) / 16u + 2ull * s <= slot;   // true for lane 0, and false from some lane on
-        const uint32_t last = (uint32_t)__popc(__ballot_sync(0xffffffffu, in)) - 1u;
+        const bool in = s < hi && begin(s) / 16u + 2ull * s <= slot;   // true up to some lane, false from there on
+        const uint32_t last = max((uint32_t)__popc(__ballot_sync(0xffffffffu, in)), 1u) - 1u;
         lo += last * step;
         hi = min(hi, lo + step);
     }
     const uint64_t b = begin(lo), e = begin(lo + 1u);
     *cut = UINT32_MAX;
-    if (e <= b) return false;
+    if (e <= b || slot < b / 16u + 2ull * lo) return false;   // (the latter: tokens in front of cu[0], nobody's)
     const uint32_t p = pos0[lo];
     const uint64_t j = slot - (b / 16u + 2ull * lo);
     const uint64_t end_all = (uint64_t)p + (e - b);

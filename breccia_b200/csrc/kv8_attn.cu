@@ -384,11 +384,13 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
                         if (mine && ok)
                             brc::tma_load_4d(base + st * STAGE + sl * (SLAB), &tm, (int32_t)(sl * 128u), (int32_t)row0,
                                              (int32_t)(p.page0 + id), 0, full0 + 8u * st, policy);
-                        stage += min(BATCH, m - i);
+                        if (ok) stage += min(BATCH, m - i);
                         if (stage >= p.n_stages) { stage -= p.n_stages; parity ^= 1u; }
                     }
                 }
             }
+            if (!ok)   // a wait ran out: the block may not end while copies into its shared memory are under way
+                for (uint32_t i = 0; i < p.n_stages; ++i) brc::mbar_wait(full0 + 8u * i, i < stage ? parity ^ 1u : parity, 1u << 16);
         }
         if (!ok && lane == 0) { atomicOr(p.status, BRC_DEV_WAIT_LIMIT); p.status[1] = blockIdx.x; }
         return;
@@ -956,7 +958,7 @@ brc_status brc_kv8_attend(brc_pool *pool, const char *who, const brc_kv8_attn_ar
     if ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.workspace)) & 15u)
         return brc_fail(BRC_ERR_INVALID, "%s: query, output and workspace pointers must be 16-byte aligned", who);
     const Shape s = shape_of(pool, a.n_seqs, a.n_head, a.max_q);
-    if ((uint64_t)a.max_q * s.group >= (1ull << 31) || (uint64_t)a.n_seqs * s.units_per_seq >= (1ull << 31))
+    if ((uint64_t)a.max_q * s.group >= (1ull << 31) || (uint64_t)(pool->n_kv_head / s.kvb) * s.passes >= (1ull << 31) || (uint64_t)a.n_seqs * s.units_per_seq >= (1ull << 31))
         return brc_fail(BRC_ERR_UNSUPPORTED, "%s: %u sequences of %u tokens with %u heads per kv head in one call", who, a.n_seqs, a.max_q, s.group);
     if (!a.workspace || a.workspace_bytes < s.workspace())
         return brc_fail(BRC_ERR_INVALID, "%s: workspace of %llu bytes, %llu needed", who, (unsigned long long)a.workspace_bytes,

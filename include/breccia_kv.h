@@ -350,7 +350,9 @@ BRC_API brc_status brc_paged_decode_attn_static(brc_pool *pool, uint32_t layer, 
  *     brc_rope_apply would with the same n_rot, rope_layout and rope_factor.
  * brc_kv8_read: cells pos0_dev[s] .. of each sequence as values, packed
  * [total_tokens][n_kv_head][head_dim] f32, f16 or bf16 (rounded once; f32 and,
- * for int8 codes, bf16 are exact unless out of range).  Outputs 16-byte aligned. */
+ * for int8 codes, bf16 are exact unless out of range).  Outputs 16-byte aligned;
+ * rows of cells past max_pos_end or of a page id out of range are left as they
+ * were, and reported. */
 #define BRC_ROPE_HALF 0        /* pairs (j, j + n_rot / 2) */
 #define BRC_ROPE_INTERLEAVED 1 /* pairs (2 j, 2 j + 1)     */
 BRC_API brc_status brc_kv8_append(brc_pool *pool, uint32_t layer, const uint32_t *block_tables_dev, uint32_t table_stride,
@@ -409,7 +411,8 @@ BRC_API brc_status brc_kv8_attn(brc_pool *pool, uint32_t layer, const void *q_de
  * brc_rope_apply: rotates q and / or k rows [n_tokens][heads][head_dim] (NULL: the
  * other alone), f32, f16 or bf16, computed in f32; dims at and past n_rot are
  * copied.  Token strides in elements, 0: packed.  An output may be its input, the
- * same rows; otherwise the two must not overlap. */
+ * same rows; otherwise the two must not overlap, and neither output may touch the
+ * other side's rows (q and k as columns of one wider row are apart). */
 #define BRC_ROPE_NONE 0
 #define BRC_ROPE_LINEAR 1
 #define BRC_ROPE_NTK 2

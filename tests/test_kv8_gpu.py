@@ -346,6 +346,56 @@ def test_long_sequences_split_over_every_sm(cuda_device, code):
     pool.release()
 
 
+def test_nothing_to_attend_to(cuda_device):
+    """Every sequence empty: zeros, whatever the workspace and the output held; no sequences, no tokens: nothing written."""
+    pool = KvPool(0, 1, 2, 128, 4, kv8="int8")
+    t, q = dev(np.zeros((5, 2))), torch.randn(10, 8, 128, device="cuda").half()
+    ws, out = kv8_workspace(pool, 5, 8, 2), torch.full((10, 8, 128), 7.0, device="cuda").half()
+    ws.fill_(255)
+    for bound in (0, 32):
+        out.fill_(7)
+        kv8_attend(pool, 0, q, t, dev([0] * 5), bound, ws, max_q=2, out=out)
+        pool.check()
+        assert (out == 0).all()
+    out.fill_(7)
+    kv8_attend(pool, 0, q, t, dev([3] * 5), 32, ws, max_q=2, cu_q=dev([0, 0, 2, 2, 2, 2]), out=out)   # four sequences without tokens, rows behind the last one
+    pool.check()
+    assert (out[:2] == 0).all() and (out[2:] == 7).all()   # (zeros: a zeroed pool)
+    assert kv8_attend(pool, 0, q[:0], t[:0], dev([]), 32, ws).shape == (0, 8, 128)
+    pool.release()
+
+
+def test_a_prefix_that_does_not_begin_at_zero(cuda_device):
+    """Tokens in front of cu_tokens[0] belong to nobody; those behind the last entry neither."""
+    pool = KvPool(0, 1, 1, 128, 8, kv8="e4m3")
+    k = torch.randn(60, 1, 128, device="cuda")
+    for first, n in ((3, 5), (40, 17), (16, 16)):
+        pool.zero()
+        kv8_append(pool, 0, k, k, dev([[4, 2]]), dev([1]), 32, cu_tokens=dev([first, first + n]))
+        pool.check()
+        got, _ = kv8_read(pool, 0, dev([[4, 2]]), dev([1]), 32, tokens_per_seq=n, dtype=torch.float32)
+        # e4m3: half a step, 2^-4 of the value, below the least normal code 2^-10 of the scale (at most 2 max / 448)
+        assert ((got - k[first:first + n]).abs() <= 2.0 ** -4 * k[first:first + n].abs() + 2.0 ** -10 * 2 * k.abs().max() / 448).all()
+        codes = pool.kv8_view(0, 0)[0].float()
+        assert codes[[0, 1, 3, 5, 6, 7]].abs().max() == 0 and codes[4, :, 0].abs().max() == 0
+    pool.release()
+
+
+def test_raw_pages_through_the_host(cuda_device):
+    """read / write move whole half pages, codes and scales."""
+    pool = KvPool(0, 1, 2, 128, 3, kv8="int8")
+    fill(pool, 3)
+    raw = pool.read(1, 0)
+    assert raw.shape == (3, pool.half_page_bytes) and pool.half_page_bytes % 128 == 0
+    codes, scales = (x.cpu().numpy() for x in pool.kv8_view(1, 0))
+    assert np.array_equal(raw[:, :2 * 16 * 128].view(np.int8).reshape(3, 2, 16, 128), codes)
+    assert np.array_equal(raw[:, 2 * 16 * 128:2 * 16 * 128 + 8].copy().view(np.float32), scales)
+    pool.zero()
+    pool.write(1, 0, raw)
+    assert np.array_equal(pool.read(1, 0), raw) and pool.bytes() == 2 * 3 * pool.half_page_bytes
+    pool.release()
+
+
 def test_many_short_sequences(cuda_device):
     """More sequences than threads in the schedule's scan, most of them a page or none, sharing pages."""
     g = np.random.default_rng(0)
