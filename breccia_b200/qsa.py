@@ -498,8 +498,8 @@ def _dtype(t: torch.dtype, who: str) -> int:
 
 def _token_rows(t: torch.Tensor, heads: int, head_dim: int, who: str) -> int:
     """Elements from one token's row [heads, head_dim] (or [heads * head_dim]) to the next; the row itself is contiguous."""
-    row = heads * head_dim
-    if t.is_contiguous() and t.dim() == 3 and t.shape[1] == heads and t.shape[2] == head_dim:
+    row, shape = heads * head_dim, t.shape
+    if t.is_contiguous() and len(shape) == 3 and shape[1] == heads and shape[2] == head_dim:
         return row
     ok = (t.dim() == 2 and t.shape[1] == row and t.stride(1) == 1) or \
          (t.dim() == 3 and t.shape[1:] == (heads, head_dim) and t.stride(2) == 1 and (heads == 1 or t.stride(1) == head_dim))
@@ -541,15 +541,21 @@ class Rope:
         self._call = _lib.load().brc_rope_apply
 
     def _side(self, name: str, x: torch.Tensor, y: torch.Tensor | None, tokens: int, hd: int, dtype: torch.dtype):
+        """(output, heads, token stride of x, of the output)"""
+        if x.dim() != 3:
+            raise BrcError(_lib.ERR_INVALID, f"Rope.apply: {name} {tuple(x.shape)}: [tokens, heads, head_dim] wanted")
+        n, heads, d = x.shape
+        if n != tokens or d != hd or x.dtype != dtype or x.get_device() != self.device:
+            raise BrcError(_lib.ERR_INVALID, f"Rope.apply: {name} {tuple(x.shape)} {x.dtype} on {x.device} beside {tokens} tokens of heads of {hd}, {dtype}, the "
+                                             f"frequencies on cuda:{self.device}")
+        row = heads * hd
+        whole = x.is_contiguous()
+        stride = row if whole else _token_rows(x, heads, hd, "Rope.apply")
         if y is None:
-            y = torch.empty_like(x, memory_format=torch.contiguous_format)
-        if x.dim() != 3 or x.shape[2] != hd or x.shape[0] != tokens or y.shape != x.shape or y.dtype != x.dtype or x.dtype != dtype:
-            raise BrcError(_lib.ERR_INVALID, f"Rope.apply: {name} {tuple(x.shape)} {x.dtype} -> {tuple(y.shape)} {y.dtype} beside {tokens} tokens of "
-                                             f"heads of {hd}, {dtype}")
-        if x.get_device() != self.device or y.get_device() != self.device:
-            raise BrcError(_lib.ERR_INVALID, f"Rope.apply: {name} on {x.device} -> {y.device}, the frequencies on cuda:{self.device}")
-        heads = x.shape[1]
-        return y, heads, _token_rows(x, heads, hd, "Rope.apply"), _token_rows(y, heads, hd, "Rope.apply")
+            return torch.empty_like(x) if whole else torch.empty(x.shape, dtype=dtype, device=x.device), heads, stride, row
+        if y.shape != x.shape or y.dtype != dtype or y.get_device() != self.device:
+            raise BrcError(_lib.ERR_INVALID, f"Rope.apply: {name} {tuple(x.shape)} {x.dtype} -> {tuple(y.shape)} {y.dtype} on {y.device}")
+        return y, heads, stride, _token_rows(y, heads, hd, "Rope.apply")
 
     def apply(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, q_out: torch.Tensor | None = None,
               k_out: torch.Tensor | None = None, stream=None):
@@ -605,7 +611,8 @@ def kv8_read(pool: KvPool, layer: int, block_tables: torch.Tensor, pos0: torch.T
     tables, at = _words(block_tables, device, "kv8_read: block_tables"), _words(pos0, device, "kv8_read: pos0", n_seqs)
     cu = None if cu_tokens is None else _words(cu_tokens, device, "kv8_read: cu_tokens", n_seqs + 1)
     code = _dtype(dtype, "kv8_read")
-    k, v = torch.empty((2, total_tokens, pool.n_kv_head, pool.head_dim), dtype=dtype, device=block_tables.device).unbind(0)
+    both = torch.empty((2, total_tokens, pool.n_kv_head, pool.head_dim), dtype=dtype, device=block_tables.device)
+    k, v = both[0], both[1]
     _lib.check(_lib.load().brc_kv8_read(pool.handle, layer, tables, stride, at, n_seqs, tokens_per_seq, cu, total_tokens, max_pos_end, k.data_ptr(),
                                         v.data_ptr(), code, _raw_stream(stream, device)))
     return k, v
