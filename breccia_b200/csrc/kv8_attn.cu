@@ -34,15 +34,6 @@
 
 namespace {
 
-#ifndef UNIT_KIB
-#define UNIT_KIB 256u
-#endif
-#ifndef KV8_W1_128
-#define KV8_W1_128 12
-#define KV8_W1_256 8
-#define KV8_W2_128 12
-#define KV8_W2_256 8
-#endif
 constexpr uint32_t PASS_ROWS = 32;       // query rows (tokens x heads of a kv head) that share one stream of the cache
 constexpr uint32_t MIN_SHARE = 4;        // page-units a CTA takes at least
 constexpr uint32_t SMEM_LIMIT = 232448;  // 227 KiB
@@ -913,7 +904,10 @@ brc_status launch(const brc_pool *pool, AttnParams p, uint32_t grid, uint32_t me
 
 template <int HD, uint32_t CODE, bool PREC, int KVB>
 brc_status launch_rows(const brc_pool *pool, const AttnParams &p, uint32_t grid, uint32_t rt, uint32_t merge_rows, cudaStream_t st) {
-    constexpr int W1 = HD == 128 ? KV8_W1_128 : KV8_W1_256, W2 = HD == 128 ? KV8_W2_128 : KV8_W2_256;
+    // Warps: what the registers of the sums allow and the ring bears (a stage for each warp that takes pages in turn, twice
+    // over).  Measured (us) at 8, 12, 16 warps of head_dim 128: 32 sequences, 8 kv heads 54.4, 51.4, 53.5; drafts of 24 sequences 50.4, 50.2,
+    // 52.4; eight tokens each 79, 73, 84.
+    constexpr int W1 = HD == 128 ? 12 : 8, W2 = W1;
     if (rt == 1) return launch<HD, CODE, PREC, 1, 1, KVB, W1>(pool, p, grid, merge_rows, st);
     return p.row_groups == 1 ? launch<HD, CODE, PREC, 2, 1, KVB, W2>(pool, p, grid, merge_rows, st) : launch<HD, CODE, PREC, 2, 2, KVB, W2>(pool, p, grid, merge_rows, st);
 }
@@ -998,8 +992,12 @@ brc_status brc_kv8_attend(brc_pool *pool, const char *who, const brc_kv8_attn_ar
     p.passes = s.passes;
     p.units_per_seq = s.units_per_seq;
     p.scale_log2 = a.scale * 1.4426950408889634f;
-    // Starting and finishing a unit takes a CTA about as long as streaming UNIT_KIB.
-    p.unit_cost = std::max(1u, (UNIT_KIB * 1024u) / (s.kvb * 2u * 16u * pool->head_dim));
+    // Starting and finishing a unit takes a CTA about as long as streaming 128 KiB for each of the unit's heads, half as much again where
+    // two row tiles of 256 columns are merged.  Measured (us): 32 sequences of 512-8192 cells, 16 heads over 2 of 256: 33.2 at half of it,
+    // 32.8, 32.9 at one and a half times; with four tokens each 70.8, 66.1, 61.8, 62.1 at 128, 256, 384, 512 KiB; 7 heads over 7 of 128: 58.5 at 128 KiB,
+    // 62.4 at 256.
+    const uint32_t unit_kib = 128u * s.kvb * (s.rt == 2u && pool->head_dim == 256 ? 3u : 2u) / 2u;
+    p.unit_cost = std::max(1u, unit_kib * 1024u / (s.kvb * 2u * 16u * pool->head_dim));
     const uint64_t most = (uint64_t)a.n_seqs * s.units_per_seq * ((a.max_seq_len + 15ull) / 16u + p.unit_cost);   // cost at most
     if (most >= (1ull << 31))
         return brc_fail(BRC_ERR_UNSUPPORTED, "%s: %u sequences of up to %u cells in %u passes each are too much for one call", who, a.n_seqs, a.max_seq_len,
