@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
         if (idx == 0) {   // the first unit's q: nobody has anything else to do yet
             // (scales asked for with the q rows: behind the first pages' boxes they would come 3 us later)
             bool asked = false;
-            stage_q<HD, PREC, 2>(p, L, smem, g, 0, warp, W, lane, [&] { scales_of(g, ids, ks_next, ev_next); asked = true; });
+            stage_q<HD, PREC, RT == 1 ? 2 : 4>(p, L, smem, g, 0, warp, W, lane, [&] { scales_of(g, ids, ks_next, ev_next); asked = true; });
             if (!asked) scales_of(g, ids, ks_next, ev_next);
             brc::named_bar_sync(1, CONSUMERS);
         } else {
@@ -633,7 +633,8 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
         if (lane == 0) brc::mbar_arrive(q_empty0 + 8u * buf_q);
         ++idx;
 
-        // ---- merge the warps that took this unit's pages in turn; finish it, or leave a partial
+        // ---- merge the warps that took this unit's pages in turn: they agree on the rows' references, bring their sums to them and
+        // add up; then the row is finished, or a partial left
 #pragma unroll
         for (int n = 0; n < RT; ++n)
 #pragma unroll
@@ -645,11 +646,29 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
                 if (gr == 0) stat[warp * 16u + n * 8u + 2u * t + x] = make_float4(m_run[n][x], w_run[n][x], l, 0.f);
             }
         const bool whole = g.n == g.pages;
-        const uint64_t slot = 2ull * blockIdx.x + (g.pg == 0 ? 1u : 0u);
+        const uint64_t slot = (2ull * blockIdx.x + (g.pg == 0 ? 1u : 0u)) * (KVB * PASS);
         more = next_segment(p, cur, g_next);
         if (more) ids = ids_of(g_next, (pl + LANES - done % LANES) % LANES);   // on their way while this unit is merged
+        brc::named_bar_sync(1, CONSUMERS);
 #pragma unroll
         for (int n = 0; n < RT; ++n) {
+            float f[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const float4 *st = stat + (warp % STEP) * 16u + n * 8u + 2u * t + x;
+                float m = NONE, wm = NONE, l = 0.f;
+#pragma unroll
+                for (uint32_t q = 0; q < LANES; ++q) {
+                    m = fmaxf(m, st[q * STEP * 16u].x);
+                    wm = fmaxf(wm, st[q * STEP * 16u].y);
+                }
+#pragma unroll
+                for (uint32_t q = 0; q < LANES; ++q) l += st[q * STEP * 16u].z * brc::fast_exp2(st[q * STEP * 16u].x - m);
+                f[x] = brc::fast_exp2(w_run[n][x] - wm);
+                if (whole) f[x] *= l == 0.f ? 0.f : brc::fast_exp2(wm - m - WEIGHT_SHIFT) / l;
+                else if (pl == 0 && gr == 0)
+                    *reinterpret_cast<float4 *>(p.ml + (slot + hk * PASS + (rg * RT + n) * 8u + 2u * t + x) * 4u) = make_float4(m, wm, l, 0.f);
+            }
 #pragma unroll
             for (uint32_t sl = 0; sl < SLABS; ++sl)
 #pragma unroll
@@ -660,62 +679,40 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
                         for (uint32_t x = 0; x < 2; ++x) {
                             const float(*a)[4] = &o[n][sl * 8u + 4u * y];
                             *reinterpret_cast<float4 *>(scratch + (warp * 8u + 2u * t + x) * ROW + 128u * sl + 16u * gr + 8u * h + 4u * y) =
-                                make_float4(a[0][2 * h + x], a[1][2 * h + x], a[2][2 * h + x], a[3][2 * h + x]);
+                                make_float4(a[0][2 * h + x] * f[x], a[1][2 * h + x] * f[x], a[2][2 * h + x] * f[x], a[3][2 * h + x] * f[x]);
                         }
             brc::named_bar_sync(1, CONSUMERS);
-            {
-                constexpr uint32_t C4 = HD / 4, U = 4;   // U groups of four values a thread side by side
-                const uint32_t items = STEP * 8u * C4;
-                for (uint32_t it0 = tid; it0 < items; it0 += U * CONSUMERS) {
-                    float m[U], wm[U], l[U], v[U][4];
-                    uint32_t at[U];   // stat row of the first warp that holds the item; 0 stands in past the end
+            constexpr uint32_t C4 = HD / 4, ITEMS = STEP * 8 * C4, IT = (ITEMS + CONSUMERS - 1) / CONSUMERS;   // groups of four values
+            const uint32_t d = tid % C4 * 4u;   // CONSUMERS is a multiple of C4
+            float4 v[IT];
 #pragma unroll
-                    for (uint32_t k = 0; k < U; ++k) {
-                        const uint32_t it = it0 + k * CONSUMERS, wg = it / (8u * C4);   // head + kvb * row group
-                        at[k] = it < items ? wg * 16u + n * 8u + it / C4 % 8u : 0u;
-                        m[k] = wm[k] = NONE;
-                        l[k] = v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0.f;
-                    }
-                    for (uint32_t q = 0; q < LANES; ++q)
+            for (uint32_t k = 0; k < IT; ++k) {
+                const uint32_t row = (tid + k * CONSUMERS) / C4;   // row of a tile + 8 * (head + kvb * row group)
+                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (ITEMS % CONSUMERS != 0 && row >= STEP * 8u) continue;
 #pragma unroll
-                        for (uint32_t k = 0; k < U; ++k) {
-                            const float4 st = stat[at[k] + q * STEP * 16u];
-                            m[k] = fmaxf(m[k], st.x);
-                            wm[k] = fmaxf(wm[k], st.y);
-                        }
-                    const uint32_t d = it0 % C4 * 4u;   // CONSUMERS is a multiple of C4
-                    for (uint32_t q = 0; q < LANES; ++q)
-#pragma unroll
-                        for (uint32_t k = 0; k < U; ++k) {
-                            const float4 st = stat[at[k] + q * STEP * 16u];
-                            const float4 x = *reinterpret_cast<const float4 *>(scratch + ((at[k] / 16u + q * STEP) * 8u + at[k] % 8u) * ROW + d);
-                            const float f = brc::fast_exp2(st.y - wm[k]);
-                            l[k] += st.z * brc::fast_exp2(st.x - m[k]);
-                            v[k][0] += x.x * f;
-                            v[k][1] += x.y * f;
-                            v[k][2] += x.z * f;
-                            v[k][3] += x.w * f;
-                        }
-#pragma unroll
-                    for (uint32_t k = 0; k < U; ++k) {
-                        const uint32_t wg = at[k] / 16u, r = ((wg / KVB) * RT + n) * 8u + at[k] % 8u, h = wg % KVB;
-                        const uint32_t gr_row = pass * PASS + r;
-                        if (it0 + k * CONSUMERS >= items || gr_row >= rows) continue;
-                        if (whole) {
-                            const float f = l[k] == 0.f ? 0.f : brc::fast_exp2(wm[k] - m[k] - WEIGHT_SHIFT) / l[k];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) v[k][e] *= f;
-                            const uint32_t tok = gr_row / p.group, head = (hg * KVB + h) * p.group + gr_row % p.group;
-                            finish_row(p, HD, (tok0 + tok) * p.n_head + head, d, v[k]);
-                        } else {
-                            const uint64_t to = slot * KVB * PASS + h * PASS + r;
-                            *reinterpret_cast<float4 *>(p.acc + to * HD + d) = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
-                            if (d == 0) *reinterpret_cast<float4 *>(p.ml + to * 4u) = make_float4(m[k], wm[k], l[k], 0.f);
-                        }
-                    }
+                for (uint32_t q = 0; q < LANES; ++q) {
+                    const float4 x = *reinterpret_cast<const float4 *>(scratch + (row + q * STEP * 8u) * ROW + d);
+                    v[k].x += x.x;
+                    v[k].y += x.y;
+                    v[k].z += x.z;
+                    v[k].w += x.w;
                 }
-                brc::named_bar_sync(1, CONSUMERS);
             }
+#pragma unroll
+            for (uint32_t k = 0; k < IT; ++k) {
+                const uint32_t row = (tid + k * CONSUMERS) / C4, wg = row / 8u, r = ((wg / KVB) * RT + n) * 8u + row % 8u, h = wg % KVB;
+                const uint32_t gr_row = pass * PASS + r;
+                if ((ITEMS % CONSUMERS != 0 && row >= STEP * 8u) || gr_row >= rows) continue;
+                if (whole) {
+                    const uint32_t tok = gr_row / p.group, head = (hg * KVB + h) * p.group + (gr_row - tok * p.group);
+                    float y[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+                    finish_row(p, HD, (tok0 + tok) * p.n_head + head, d, y);
+                } else {
+                    *reinterpret_cast<float4 *>(p.acc + (slot + h * PASS + r) * HD + d) = v[k];
+                }
+            }
+            brc::named_bar_sync(1, CONSUMERS);
         }
         g = g_next;
     }
