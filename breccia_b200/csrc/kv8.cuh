@@ -142,6 +142,13 @@ __device__ __forceinline__ void load8(const typename elem<DT>::t *p, bool vec, f
     }
 }
 
+// The larger of a magnitude, given as bits, and |x|; NaN wins (the bits of one are above those of infinity).
+__device__ __forceinline__ uint32_t max_magnitude(uint32_t m, float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(m)), "f"(fabsf(x)));
+    return __float_as_uint(r);
+}
+
 // Eight consecutive elements as they lie in memory: half the registers of their f32 values for the 16-bit types.
 template <int DT>
 struct raw8 {
@@ -190,7 +197,7 @@ struct raw8 {
     __device__ __forceinline__ void top(uint32_t &m) const {
 #pragma unroll
         for (int i = 0; i < WORDS; ++i) {
-            if constexpr (DT == 0) m = max(m, w[i] & 0x7fffffffu);
+            if constexpr (DT == 0) m = max_magnitude(m, __uint_as_float(w[i]));
             else asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7fff7fffu));
         }
     }

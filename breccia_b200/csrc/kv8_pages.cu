@@ -61,9 +61,10 @@ __device__ __forceinline__ void rotate8(const PagesParams &p, const typename brc
     } else if (half % 8u == 0u) {   // a chunk lies in one half, its partners are the chunk half / 8 lanes away
         const bool second = d >= half;
         const uint32_t lane = threadIdx.x & 31u, from = d >= p.n_rot ? lane : second ? lane - half / 8u : lane + half / 8u;
-        brc::raw8<DT> other;
+        brc::raw8<DT> other;   // of the first half: negated, (x c - y s); of the second: (y c + x s)
+        const uint32_t sign = second ? 0u : DT == 0 ? 0x80000000u : 0x80008000u;
 #pragma unroll
-        for (int j = 0; j < brc::raw8<DT>::WORDS; ++j) other.w[j] = __shfl_sync(0xffffffffu, raw.w[j], from);
+        for (int j = 0; j < brc::raw8<DT>::WORDS; ++j) other.w[j] = __shfl_sync(0xffffffffu, raw.w[j], from) ^ sign;
         if (d < p.n_rot) {
             float o[8];
             other.values(o);
@@ -71,8 +72,8 @@ __device__ __forceinline__ void rotate8(const PagesParams &p, const typename brc
 #pragma unroll
             for (uint32_t j = 0; j < 8; j += 2) {
                 const float4 a = a4[j / 2u];
-                v[j] = second ? o[j] * a.y + v[j] * a.x : v[j] * a.x - o[j] * a.y;
-                v[j + 1] = second ? o[j + 1] * a.w + v[j + 1] * a.z : v[j + 1] * a.z - o[j + 1] * a.w;
+                v[j] = v[j] * a.x + o[j] * a.y;
+                v[j + 1] = v[j + 1] * a.z + o[j + 1] * a.w;
             }
         }
     } else if (live) {
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(128, append_ctas(DT, HD, ROPE)) kv8_append_ker
                 raw[i].values(v[i]);
                 rotate8<DT, HD>(p, src + (r * stride + h * HD), cos_sin + (r < t.count ? r : 0u) * half, d, r < t.count, raw[i], v[i]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+                for (int j = 0; j < 8; ++j) top = brc::max_magnitude(top, v[i][j]);
             }
         } else {
 #pragma unroll
