@@ -144,12 +144,12 @@ SIGNATURES = {
     "brc_paged_sparse_attn": [_vp, _u32, _vp, _i32, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _vp, _u32, _f32, _vp, _vp],
     "brc_pool_create_kv8": [_i32, _u32, _u32, _u32, _u32, _u32, _i32, _vpp],
     "brc_pool_kv8_code": [_vp, C.POINTER(C.c_int32)],
-    "brc_kv8_append": [_vp, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _u32, _vp, _u64, _vp, _u64, _i32, _vp, _u32, _i32, _f32, _vp],
+    "brc_kv8_append": [_vp, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _u32, _vp, _u64, _vp, _u64, _i32, _vp, _u32, _i32, C.c_double, _vp],
     "brc_kv8_read": [_vp, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _u32, _vp, _vp, _i32, _vp],
     "brc_kv8_attn_workspace_bytes": [_vp, _u32, _u32, _u32, _u64p],
     "brc_kv8_attn": [_vp, _u32, _vp, _i32, _u32, _vp, _u32, _vp, _u32, _vp, _vp, _u32, _u32, _u32, _f32, _vp, _i32, _vp, _u64, _vp],
-    "brc_rope_freqs": [C.POINTER(RopeParams), _u64p, C.POINTER(C.c_float)],
-    "brc_rope_apply": [_i32, _vp, _vp, _u32, _u64, _u64, _vp, _vp, _u32, _u64, _u64, _u32, _i32, _vp, _u32, _vp, _u32, _i32, _f32, _vp],
+    "brc_rope_freqs": [C.POINTER(RopeParams), _u64p, C.POINTER(C.c_double)],
+    "brc_rope_apply": [_i32, _vp, _vp, _u32, _u64, _u64, _vp, _vp, _u32, _u64, _u64, _u32, _i32, _vp, _u32, _vp, _u32, _i32, C.c_double, _vp],
     "brc_timing_enable": [_vp, _i32],
     "brc_timing_read": [_vp, _i32, _u32p, C.POINTER(C.c_double)],
 }

@@ -241,12 +241,14 @@ __device__ __forceinline__ void store8(typename elem<DT>::t *p, bool vec, const 
 // ---------------------------------------------------------------------------------------------
 // Turns per position as a 0.64 fixed-point fraction: pos * turns modulo 2^64 IS the fraction of a turn (whole turns
 // fall off the top), off by at most pos * 2^-65, where an f32 angle of position 10^6 has lost 16 of its 24 bits.
-// Read as a signed number it lies in [-1/2, 1/2) turns; times two that is sincospi's argument.
-__device__ __forceinline__ float2 rope_cos_sin(uint32_t pos, uint64_t turns, float factor) {
+// Read as a signed number it lies in [-1/2, 1/2) turns; times two that is sincospi's argument.  Sine, cosine and the factor
+// in 64 bits and one rounding to f32: a pair is computed once for all heads of a token, and a wrong last bit of it
+// shows as a neighbouring 8-bit code wherever a rotated key lies on a border.
+__device__ __forceinline__ float2 rope_cos_sin(uint32_t pos, uint64_t turns, double factor) {
     const int64_t f = (int64_t)((uint64_t)pos * turns);
-    float s, c;
-    sincospif((float)f * 0x1p-63f, &s, &c);
-    return make_float2(c * factor, s * factor);
+    double s, c;
+    sincospi((double)f * 0x1p-63, &s, &c);
+    return make_float2((float)(c * factor), (float)(s * factor));
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -27,7 +27,7 @@ struct PagesParams {
     uint64_t page_bytes;
     uint32_t table_stride, n_seqs, tokens_per_seq, total_tokens, max_pos_end, n_pages, n_kv_head, heads_per_cta;
     uint32_t n_rot, interleaved;
-    float factor;
+    double factor;
     bool k_vec, v_vec;
 };
 
@@ -337,7 +337,7 @@ brc_status brc_kv8_append(brc_pool *pool, uint32_t layer, const uint32_t *block_
                           const uint32_t *pos0_dev, uint32_t n_seqs, uint32_t tokens_per_seq, const uint32_t *cu_tokens_dev,
                           uint32_t total_tokens, uint32_t max_pos_end, const void *k_src_dev, uint64_t k_token_stride,
                           const void *v_src_dev, uint64_t v_token_stride, int32_t src_dtype, const uint64_t *rope_turns_dev,
-                          uint32_t n_rot, int32_t rope_layout, float rope_factor, void *stream) {
+                          uint32_t n_rot, int32_t rope_layout, double rope_factor, void *stream) {
     const char *who = "brc_kv8_append";
     bool go;
     if (brc_status rc = validate(pool, who, "write", layer, block_tables_dev, table_stride, pos0_dev, n_seqs, tokens_per_seq,

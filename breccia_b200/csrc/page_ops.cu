@@ -223,7 +223,7 @@ brc_status brc_kv_append(brc_pool *pool, uint32_t layer, const uint32_t *block_t
         if (src_dtype != BRC_DTYPE_F32 && src_dtype != BRC_DTYPE_F16)
             return brc_fail(BRC_ERR_INVALID, "brc_kv_append: src_dtype %d is neither f32 (0) nor f16 (1)", src_dtype);
         return brc_kv8_append(pool, layer, block_tables_dev, table_stride, pos0_dev, n_seqs, tokens_per_seq, cu_tokens_dev, total_tokens,
-                              max_pos_end, k_src_dev, 0, v_src_dev, 0, src_dtype, nullptr, 0, BRC_ROPE_HALF, 1.f, stream);
+                              max_pos_end, k_src_dev, 0, v_src_dev, 0, src_dtype, nullptr, 0, BRC_ROPE_HALF, 1.0, stream);
     }
     if (pool->v_q8 && src_dtype != BRC_DTYPE_F32)
         return brc_fail(BRC_ERR_UNSUPPORTED, "brc_kv_append: a q8_0 V pool quantises from f32 sources only (src_dtype %d)", src_dtype);

@@ -29,7 +29,7 @@ struct RopeParams {
     const uint32_t *positions;
     const uint64_t *turns;
     uint32_t n_tokens, tokens_per_cta, splits, head_dim, n_rot, interleaved;
-    float factor;
+    double factor;
 };
 
 // Sixteen bytes of a row in f32.
@@ -256,7 +256,7 @@ void launch(RopeParams &p, bool rows, uint32_t total_heads, int sm_count, cudaSt
 
 extern "C" {
 
-brc_status brc_rope_freqs(const brc_rope_params *a, uint64_t *out_turns, float *out_factor) {
+brc_status brc_rope_freqs(const brc_rope_params *a, uint64_t *out_turns, double *out_factor) {
     const char *who = "brc_rope_freqs";
     if (!a || !out_turns || !out_factor) return brc_fail(BRC_ERR_INVALID, "%s: NULL argument", who);
     if (a->n_rot == 0 || a->n_rot % 2u || a->n_rot > 256u)
@@ -294,14 +294,14 @@ brc_status brc_rope_freqs(const brc_rope_params *a, uint64_t *out_turns, float *
         }
         out_turns[j] = (uint64_t)(f / two_pi * 0x1p64L + 0.5L);   // f <= 1: below 0.16 turns
     }
-    *out_factor = a->mscale > 0.0 ? (float)a->mscale : a->scaling == BRC_ROPE_YARN ? (float)(0.1 * std::log(a->factor) + 1.0) : 1.f;
+    *out_factor = a->mscale > 0.0 ? a->mscale : a->scaling == BRC_ROPE_YARN ? 0.1 * std::log(a->factor) + 1.0 : 1.0;
     return BRC_OK;
 }
 
 brc_status brc_rope_apply(int32_t device, const void *q_dev, void *q_out_dev, uint32_t n_head, uint64_t q_token_stride,
                           uint64_t q_out_token_stride, const void *k_dev, void *k_out_dev, uint32_t n_kv_head, uint64_t k_token_stride,
                           uint64_t k_out_token_stride, uint32_t head_dim, int32_t dtype, const uint32_t *positions_dev,
-                          uint32_t n_tokens, const uint64_t *turns_dev, uint32_t n_rot, int32_t layout, float factor, void *stream) {
+                          uint32_t n_tokens, const uint64_t *turns_dev, uint32_t n_rot, int32_t layout, double factor, void *stream) {
     const char *who = "brc_rope_apply";
     if (dtype != BRC_DTYPE_F32 && dtype != BRC_DTYPE_F16 && dtype != BRC_DTYPE_BF16)
         return brc_fail(BRC_ERR_INVALID, "%s: dtype %d is none of f32 (0), f16 (1), bf16 (2)", who, dtype);

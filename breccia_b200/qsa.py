@@ -533,7 +533,7 @@ class Rope:
         a = _lib.RopeParams(theta=theta, factor=factor, turns_low=turns_low, turns_high=turns_high, mscale=mscale, n_rot=n_rot,
                             orig_ctx=orig_ctx, scaling=_lib.ROPE_SCALINGS[scaling])
         self.turns_host = np.zeros(max(n_rot // 2, 1), np.uint64)   # fractions of a turn per position, times 2^64
-        f = C.c_float()
+        f = C.c_double()
         _lib.call("brc_rope_freqs", C.byref(a), self.turns_host.ctypes.data_as(C.POINTER(C.c_uint64)), C.byref(f))
         self.factor, self.n_rot, self.layout, self.device = f.value, n_rot, _lib.ROPE_LAYOUTS[layout], device
         self.turns = torch.from_numpy(self.turns_host.view(np.int64)).to(f"cuda:{device}") if torch.cuda.is_available() else None

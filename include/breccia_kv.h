@@ -360,7 +360,7 @@ BRC_API brc_status brc_kv8_append(brc_pool *pool, uint32_t layer, const uint32_t
                                   const uint32_t *cu_tokens_dev, uint32_t total_tokens, uint32_t max_pos_end,
                                   const void *k_src_dev, uint64_t k_token_stride, const void *v_src_dev,
                                   uint64_t v_token_stride, int32_t src_dtype, const uint64_t *rope_turns_dev,
-                                  uint32_t n_rot, int32_t rope_layout, float rope_factor, void *stream);
+                                  uint32_t n_rot, int32_t rope_layout, double rope_factor, void *stream);
 BRC_API brc_status brc_kv8_read(brc_pool *pool, uint32_t layer, const uint32_t *block_tables_dev, uint32_t table_stride,
                                 const uint32_t *pos0_dev, uint32_t n_seqs, uint32_t tokens_per_seq,
                                 const uint32_t *cu_tokens_dev, uint32_t total_tokens, uint32_t max_pos_end,
@@ -380,6 +380,8 @@ BRC_API brc_status brc_kv8_read(brc_pool *pool, uint32_t layer, const uint32_t *
  * Up to 32 rows (T x heads per kv head) share one stream of the cache; more are
  * taken in passes of 32, each streaming it again: made for decode and drafts,
  * not for long prompts.
+ * Same arguments, same bits; where a sequence's pages are cut between SMs, and
+ * with it the order of the f32 sums, depends on the whole batch.
  * workspace_dev: brc_kv8_attn_workspace_bytes() for these n_seqs, n_head, max_q;
  * 16-byte aligned, contents undefined before and after.  Nothing outside it is
  * shared between calls: calls with workspaces of their own may run at the same
@@ -409,7 +411,8 @@ BRC_API brc_status brc_kv8_attn(brc_pool *pool, uint32_t layer, const void *q_de
  *   BANDS   f between f and f / factor by the pair's number of turns over orig_ctx
  * mscale > 0 replaces the scaling's own factor.
  * brc_rope_apply: rotates q and / or k rows [n_tokens][heads][head_dim] (NULL: the
- * other alone), f32, f16 or bf16, computed in f32; dims at and past n_rot are
+ * other alone), f32, f16 or bf16, computed in f32 (angles, sines and the factor in
+ * 64 bits); dims at and past n_rot are
  * copied.  Token strides in elements, 0: packed.  An output may be its input, the
  * same rows; otherwise the two must not overlap, and neither output may touch the
  * other side's rows (q and k as columns of one wider row are apart). */
@@ -429,13 +432,13 @@ typedef struct brc_rope_params {
     int32_t scaling;
     int32_t reserved;
 } brc_rope_params;
-BRC_API brc_status brc_rope_freqs(const brc_rope_params *params, uint64_t *out_turns, float *out_factor);
+BRC_API brc_status brc_rope_freqs(const brc_rope_params *params, uint64_t *out_turns, double *out_factor);
 BRC_API brc_status brc_rope_apply(int32_t device, const void *q_dev, void *q_out_dev, uint32_t n_head,
                                   uint64_t q_token_stride, uint64_t q_out_token_stride, const void *k_dev,
                                   void *k_out_dev, uint32_t n_kv_head, uint64_t k_token_stride,
                                   uint64_t k_out_token_stride, uint32_t head_dim, int32_t dtype,
                                   const uint32_t *positions_dev, uint32_t n_tokens, const uint64_t *turns_dev,
-                                  uint32_t n_rot, int32_t layout, float factor, void *stream);
+                                  uint32_t n_rot, int32_t layout, double factor, void *stream);
 
 /* ---------------------------------------------------------------- split-KV across GPUs
  * One long sequence whose cells are split into contiguous, page-aligned ranges

@@ -396,6 +396,32 @@ def test_raw_pages_through_the_host(cuda_device):
     pool.release()
 
 
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_offsets_past_32_bits(cuda_device, code):
+    """A layer of more than 2^32 bytes: the same tokens in its first and its last pages, in the second of two layers."""
+    n_pages = 300_000
+    pool = KvPool(0, 2, 4, 256, n_pages, kv8=code)
+    assert n_pages * pool.half_page_bytes > 2 ** 32
+    t = dev([[3, 1, 2], [n_pages - 1, n_pages - 3, n_pages - 2]])
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (random_rows(g, 40, 4, 256, "f16").repeat(2, 1, 1) for _ in range(2))
+    kv8_append(pool, 1, k, v, t, dev([0, 0]), 40, tokens_per_seq=40)
+    got = kv8_read(pool, 1, t, dev([0, 0]), 40, tokens_per_seq=40, dtype=torch.float32)
+    assert all(torch.equal(x[:40], x[40:]) and x.abs().max() > 0 for x in got)
+    q = torch.randn(1, 8, 256, device="cuda").repeat(2, 1, 1)
+    out = kv8_attend(pool, 1, q, t, dev([40, 40]), 48, kv8_workspace(pool, 2, 8))
+    want, mag, dot = ref.attention(q[0].double().cpu().numpy(), *(x[:40].double().cpu().numpy() for x in got), 40, 1 / 16)
+    # As in the serving run; and random rows this unlike in size leave columns whose heaviest cells have code 0, where what counts lies below
+    # the least weight.  A weight is 2^(s + e_v - M + 7) in binary16, whose half spacing at zero is 2^-25, and the references lie at or
+    # under the true maxima (so the denominator is at least 1): a cell loses at most 2^-32 of a code times 2^M, 2^M at most the largest
+    # scale, and the largest code times that scale at most twice the largest value: 2^-31 max|v| a cell.
+    floor = 40 * 2.0 ** -31 * float(got[1].abs().max())
+    for row in out.double().cpu().numpy():   # (the two sequences are cut at different pages, so their f32 sums run in different orders)
+        assert (np.abs(row - want) <= mag * 2.0 ** -17 * (1 + dot[:, None]) + floor).all()
+    pool.check()
+    pool.release()
+
+
 def test_many_short_sequences(cuda_device):
     """More sequences than threads in the schedule's scan, most of them a page or none, sharing pages."""
     g = np.random.default_rng(0)

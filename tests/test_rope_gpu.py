@@ -86,6 +86,20 @@ def test_columns_of_one_projection_in_place(cuda_device, layout, offset):
     assert torch.equal(q, qs) and torch.equal(k, ks) and torch.equal(rest, rest0)
 
 
+def test_offsets_past_32_bits(cuda_device):
+    """More than 2^32 values, rotated in place: the last tokens as by themselves."""
+    tokens = 2 ** 21 + 3
+    x = torch.zeros(tokens, 16, 128, dtype=torch.float16, device="cuda")
+    x[-5:] = torch.randn(5, 16, 128, device="cuda")
+    x[0] = 1
+    last, first = x[-5:].clone(), x[:1].clone()
+    pos = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    rope = Rope(128, layout="interleaved")
+    rope.apply(x, None, pos, q_out=x)
+    assert torch.equal(x[-5:], rope.apply(last, None, pos[-5:].contiguous())[0]) and torch.equal(x[:1], first)
+    assert x[1:-5].abs().max() == 0
+
+
 def test_relative_positions(cuda_device):
     """The dot product of rotated q and k depends on the distance alone, at far positions too."""
     rope = Rope(128, theta=THETA, layout="interleaved")
