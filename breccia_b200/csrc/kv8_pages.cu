@@ -90,8 +90,8 @@ __device__ __forceinline__ void rotate8(const PagesParams &p, const typename brc
 }
 
 // CTAs an SM that the compiler has to leave registers for: more of them hide the loads and barriers of one another until the
-// registers spill.  16 384 tokens, measured: 8 heads of 128, bf16, rotated 37.7 us at 8, 40.1 at 6, 42.9 at 5; 2 heads of 256, rotated
-// f16 25.7 at 5, 28.5 at 4, f32 29.7 at 4, 36.9 at 5.
+// registers spill.  16 000 tokens, rotated, measured: 8 heads of 128, bf16, 34.1 us at 8, 35.4 at 7; 2 heads of 256, f16 22.7 at 5,
+// 24.6 at 4, f32 28.2 at 4, 31.6 at 3 (at 5, before sine and cosine went to 64 bits, 36.9 against 29.7 at 4).
 constexpr int append_ctas(int dt, int hd, bool rope) { return hd == 128 ? (rope ? (dt == 0 ? 6 : 8) : 9) : dt == 0 ? 4 : rope ? 5 : 6; }
 
 template <uint32_t CODE, int DT, int HD, bool ROPE>
