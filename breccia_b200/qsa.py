@@ -505,7 +505,11 @@ def _token_rows(t: torch.Tensor, heads: int, head_dim: int, who: str) -> int:
          (t.dim() == 3 and t.shape[1:] == (heads, head_dim) and t.stride(2) == 1 and (heads == 1 or t.stride(1) == head_dim))
     if not ok:
         raise BrcError(_lib.ERR_INVALID, f"{who}: {tuple(t.shape)} with strides {t.stride()} is not rows of {heads} x {head_dim} values")
-    return t.stride(0) if t.shape[0] > 1 else row
+    if t.shape[0] <= 1:
+        return row
+    if t.stride(0) < row:   # one row for all tokens (stride 0, which the library takes for packed rows), or overlapping ones
+        raise BrcError(_lib.ERR_INVALID, f"{who}: {tuple(t.shape)} with strides {t.stride()}: tokens share memory")
+    return t.stride(0)
 
 
 def _words(t: torch.Tensor, device: int, who: str, n: int | None = None) -> int:

@@ -66,6 +66,19 @@ def test_rope_apply_refusals():
     assert call(n=0) == 0
 
 
+def test_rows_that_share_memory_are_refused():
+    """A token broadcast over a batch has stride 0, which would be read as packed rows: past its end."""
+    from breccia_b200.qsa import _token_rows
+
+    wide = torch.zeros(4, 3 * 2 * 64)
+    assert _token_rows(wide[:, 128:256].unflatten(1, (2, 64)), 2, 64, "x") == 384
+    assert _token_rows(torch.zeros(1, 2, 64).expand(1, 2, 64), 2, 64, "x") == 128
+    for bad in (torch.zeros(1, 2, 64).expand(4, 2, 64), torch.zeros(1, 128).expand(4, 128), torch.zeros(4, 1, 64).expand(4, 2, 64),
+                torch.zeros(1024).as_strided((4, 2, 64), (64, 64, 1)), torch.zeros(1, 1, 64).expand(4, 1, 64)):
+        with pytest.raises(_lib.BrcError):
+            _token_rows(bad, bad.shape[1] if bad.dim() == 3 else 2, 64, "x")
+
+
 def test_pool_refusals():
     L = _lib.load()
     h = C.c_void_p()
