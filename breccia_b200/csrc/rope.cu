@@ -252,6 +252,18 @@ void launch(RopeParams &p, bool rows, uint32_t total_heads, int sm_count, cudaSt
     rope_any_kernel<DT><<<(p.n_tokens + p.tokens_per_cta - 1u) / p.tokens_per_cta, 256, smem, st>>>(p);
 }
 
+struct Rows {   // n of them: `bytes` each, from `at`, `stride` bytes apart
+    uint64_t at, stride, bytes;
+};
+
+// No byte of a's rows is one of b's: other ranges, or other columns of rows that are wider than both.
+bool apart(const Rows &a, const Rows &b, uint32_t n) {
+    if (a.at + (n - 1u) * a.stride + a.bytes <= b.at || b.at + (n - 1u) * b.stride + b.bytes <= a.at) return true;
+    if (n == 1u || a.stride != b.stride) return false;
+    const uint64_t s = a.stride, d = b.at >= a.at ? (b.at - a.at) % s : (s - (a.at - b.at) % s) % s;
+    return d >= a.bytes && d + b.bytes <= s;
+}
+
 }  // namespace
 
 extern "C" {
@@ -335,17 +347,24 @@ brc_status brc_rope_apply(int32_t device, const void *q_dev, void *q_out_dev, ui
                             (unsigned long long)r.out_stride, (unsigned long long)row);
         const uintptr_t at = reinterpret_cast<uintptr_t>(in[s]) | reinterpret_cast<uintptr_t>(out[s]);
         if (at & (size - 1u)) return brc_fail(BRC_ERR_INVALID, "%s: pointers must be multiples of the element size", who);
-        // in place means the same rows; rows that overlap in any other way would be read after they were written
-        if (n_tokens) {
-            const uint64_t a0 = reinterpret_cast<uintptr_t>(in[s]), a1 = a0 + ((n_tokens - 1) * r.in_stride + row) * size;
-            const uint64_t b0 = reinterpret_cast<uintptr_t>(out[s]), b1 = b0 + ((n_tokens - 1) * r.out_stride + row) * size;
-            if (a0 < b1 && b0 < a1 && !(a0 == b0 && r.in_stride == r.out_stride))
-                return brc_fail(BRC_ERR_INVALID, "%s: %s and its output overlap without being the same rows", who, s ? "k" : "q");
-        }
         rows = rows && ((at | (r.in_stride * size) | (r.out_stride * size)) & 15u) == 0;
         total_heads += heads[s];
     }
     if (n_tokens == 0) return BRC_OK;
+    // in place means the same rows; rows that overlap in any other way would be read after they were written
+    for (int s = 0; s < 2; ++s) {
+        const RopeSide &r = p.side[s], &other = p.side[1 - s];
+        if (!r.in) continue;
+        const Rows x{reinterpret_cast<uintptr_t>(r.in), r.in_stride * size, (uint64_t)r.heads * head_dim * size};
+        const Rows y{reinterpret_cast<uintptr_t>(r.out), r.out_stride * size, x.bytes};
+        if (!(x.at == y.at && (x.stride == y.stride || n_tokens == 1)) && !apart(x, y, n_tokens))
+            return brc_fail(BRC_ERR_INVALID, "%s: %s and its output overlap without being the same rows", who, s ? "k" : "q");
+        if (!other.in) continue;
+        const Rows u{reinterpret_cast<uintptr_t>(other.in), other.in_stride * size, (uint64_t)other.heads * head_dim * size};
+        const Rows w{reinterpret_cast<uintptr_t>(other.out), other.out_stride * size, u.bytes};
+        if (!apart(y, u, n_tokens) || !apart(y, w, n_tokens))
+            return brc_fail(BRC_ERR_INVALID, "%s: the output of %s overlaps the rows of %s", who, s ? "k" : "q", s ? "q" : "k");
+    }
     if (!positions_dev || !turns_dev) return brc_fail(BRC_ERR_INVALID, "%s: NULL position or frequency pointer", who);
     brc_device_guard guard(device);
     if (!guard.ok) return brc_fail(BRC_ERR_CUDA, "%s: cannot make device %d current", who, device);

@@ -415,7 +415,7 @@ BRC_API brc_status brc_kv8_attn(brc_pool *pool, uint32_t layer, const void *q_de
  * 64 bits); dims at and past n_rot are
  * copied.  Token strides in elements, 0: packed.  An output may be its input, the
  * same rows; otherwise the two must not overlap, and neither output may touch the
- * other side's rows (q and k as columns of one wider row are apart). */
+ * other side's rows (columns of one wider row are apart): refused. */
 #define BRC_ROPE_NONE 0
 #define BRC_ROPE_LINEAR 1
 #define BRC_ROPE_NTK 2

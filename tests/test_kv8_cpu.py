@@ -66,6 +66,32 @@ def test_rope_apply_refusals():
     assert call(n=0) == 0
 
 
+def test_rope_outputs_that_touch_other_rows_are_refused():
+    """Pointers are compared before any device is touched: with a NULL position pointer a call that passes that check fails at the next."""
+    L = _lib.load()
+    turns = (C.c_uint64 * 32)()
+
+    def overlap(q, qo, k, ko, qs=0, qos=0, ks=0, kos=0, n=4, q_heads=4):   # heads of 64 in f32: 256 bytes each
+        rc = L.brc_rope_apply(0, q, qo, q_heads, qs, qos, k, ko, 2 if k else 0, ks, kos, 64, 0, None, n, C.cast(turns, C.c_void_p), 64, 0, 1.0, None)
+        assert rc == _lib.ERR_INVALID
+        return b"overlap" in L.brc_last_error()
+
+    a, b = 1 << 20, 2 << 20
+    assert not overlap(a, a, b, b) and not overlap(a, a + 4096, b, b + 2048)
+    assert overlap(a, a + 256, None, None) and overlap(a, a + 4092, None, None) and overlap(a, a, None, None, qs=512)
+    assert not overlap(a, a, None, None, qs=512, n=1)
+    wide = dict(qs=512, qos=512, ks=512, kos=512)                          # 2048 bytes a token: q 1024, k 512, the rest
+    assert not overlap(a, a, a + 1024, a + 1024, **wide)                   # both in place, side by side
+    assert not overlap(a, b, a + 1024, b + 1024, **wide)
+    assert not overlap(a, a, a + 1024, a + 1536, **wide)                   # k to columns of its own
+    assert overlap(a, a, a + 768, a + 1024, **wide)                        # k's rows are q's last head
+    assert overlap(a, b, b + 512, b + 1536, **wide)                        # q's output ends inside k
+    assert overlap(a, b, a + 1024, b + 2048 * 3 + 512, **wide)             # in the last row alone
+    assert overlap(a, b, a + 1024, b + 1792, **wide)                       # k's output ends in q's next row
+    assert overlap(a, b, b, b, ks=512, kos=512) and overlap(a, b, a + 1024, b, **wide)
+    assert overlap(a, b + 1024, b, b, n=1) is False and overlap(a, b, b, b, n=1)
+
+
 def test_rows_that_share_memory_are_refused():
     """A token broadcast over a batch has stride 0, which would be read as packed rows: past its end."""
     from breccia_b200.qsa import _token_rows
