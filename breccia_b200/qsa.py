@@ -489,6 +489,14 @@ def _raw_stream(stream, device: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
 
 
+def _new(stream, make):
+    """make(), in memory of the stream that will write it (the current one's may still be in use by what runs there)."""
+    if stream is None:
+        return make()
+    with torch.cuda.stream(stream):
+        return make()
+
+
 def _dtype(t: torch.dtype, who: str) -> int:
     code = _DTYPES.get(t)
     if code is None:
@@ -544,7 +552,7 @@ class Rope:
         self._turns_ptr = self.turns.data_ptr() if self.turns is not None else None
         self._call = _lib.load().brc_rope_apply
 
-    def _side(self, name: str, x: torch.Tensor, y: torch.Tensor | None, tokens: int, hd: int, dtype: torch.dtype):
+    def _side(self, name: str, x: torch.Tensor, y: torch.Tensor | None, tokens: int, hd: int, dtype: torch.dtype, to):
         """(output, heads, token stride of x, of the output)"""
         if x.dim() != 3:
             raise BrcError(_lib.ERR_INVALID, f"Rope.apply: {name} {tuple(x.shape)}: [tokens, heads, head_dim] wanted")
@@ -556,7 +564,7 @@ class Rope:
         whole = x.is_contiguous()
         stride = row if whole else _token_rows(x, heads, hd, "Rope.apply")
         if y is None:
-            return torch.empty_like(x) if whole else torch.empty(x.shape, dtype=dtype, device=x.device), heads, stride, row
+            return _new(to, lambda: torch.empty_like(x) if whole else torch.empty(x.shape, dtype=dtype, device=x.device)), heads, stride, row
         if y.shape != x.shape or y.dtype != dtype or y.get_device() != self.device:
             raise BrcError(_lib.ERR_INVALID, f"Rope.apply: {name} {tuple(x.shape)} {x.dtype} -> {tuple(y.shape)} {y.dtype} on {y.device}")
         return y, heads, stride, _token_rows(y, heads, hd, "Rope.apply")
@@ -566,11 +574,11 @@ class Rope:
         """q [tokens, n_head, head_dim], k [tokens, n_kv, head_dim] or None, positions [tokens] int32 -> (q_out, k_out), new
         tensors unless given (q_out=q rotates in place).  Tokens may be strided (columns of one projection)."""
         tokens, hd, dtype = q.shape[0], q.shape[-1], q.dtype
-        qo, qh, qs, qos = self._side("q", q, q_out, tokens, hd, dtype)
+        qo, qh, qs, qos = self._side("q", q, q_out, tokens, hd, dtype, stream)
         if k is None:
             ko, k_ptr, ko_ptr, kh, ks, kos = None, None, None, 0, 0, 0
         else:
-            ko, kh, ks, kos = self._side("k", k, k_out, tokens, hd, dtype)
+            ko, kh, ks, kos = self._side("k", k, k_out, tokens, hd, dtype, stream)
             k_ptr, ko_ptr = k.data_ptr(), ko.data_ptr()
         at = _words(positions, self.device, "Rope.apply: positions", tokens)
         _lib.check(self._call(self.device, q.data_ptr(), qo.data_ptr(), qh, qs, qos, k_ptr, ko_ptr, kh, ks, kos, hd,
@@ -615,7 +623,7 @@ def kv8_read(pool: KvPool, layer: int, block_tables: torch.Tensor, pos0: torch.T
     tables, at = _words(block_tables, device, "kv8_read: block_tables"), _words(pos0, device, "kv8_read: pos0", n_seqs)
     cu = None if cu_tokens is None else _words(cu_tokens, device, "kv8_read: cu_tokens", n_seqs + 1)
     code = _dtype(dtype, "kv8_read")
-    both = torch.empty((2, total_tokens, pool.n_kv_head, pool.head_dim), dtype=dtype, device=block_tables.device)
+    both = _new(stream, lambda: torch.empty((2, total_tokens, pool.n_kv_head, pool.head_dim), dtype=dtype, device=block_tables.device))
     k, v = both[0], both[1]
     _lib.check(_lib.load().brc_kv8_read(pool.handle, layer, tables, stride, at, n_seqs, tokens_per_seq, cu, total_tokens, max_pos_end, k.data_ptr(),
                                         v.data_ptr(), code, _raw_stream(stream, device)))
@@ -648,7 +656,7 @@ def kv8_attend(pool: KvPool, layer: int, q: torch.Tensor, block_tables: torch.Te
     else:
         cu = None
     if out is None:
-        out = torch.empty_like(q) if out_dtype is None else torch.empty_like(q, dtype=out_dtype)
+        out = _new(stream, lambda: torch.empty_like(q, dtype=out_dtype))
     elif out.shape != q.shape or not out.is_contiguous() or out.get_device() != device:
         raise BrcError(_lib.ERR_INVALID, f"kv8_attend: out {tuple(out.shape)} on {out.device} beside q {tuple(q.shape)}")
     if workspace.get_device() != device or (gate is not None and (gate.get_device() != device or gate.dtype != torch.float32)):

@@ -534,6 +534,31 @@ def test_two_streams_and_two_graphs_side_by_side(cuda_device):
     pool.release()
 
 
+def test_outputs_belong_to_the_stream_that_writes_them(cuda_device):
+    """An output made for a call on another stream must not come from memory that the current stream may still use."""
+    pool = KvPool(0, 1, 2, 128, 4, kv8="int8")
+    fill(pool, 3)
+    t, n, zero = dev([[0, 1]]), dev([20]), dev([0])
+    q, ws, rope, pos = torch.randn(1, 4, 128, device="cuda"), kv8_workspace(pool, 1, 4), Rope(128), dev([5])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for call in (lambda: kv8_read(pool, 0, t, zero, 20, 20, stream=side)[0], lambda: kv8_attend(pool, 0, q, t, n, 20, ws, stream=side),
+                 lambda: rope.apply(q, None, pos, stream=side)[0]):
+        out = call()
+        shape, where = out.shape, out.data_ptr()
+        side.synchronize()
+        del out
+        with torch.cuda.stream(side):
+            back = call()                     # the block that was just given up: it is the side stream's
+        assert back.data_ptr() == where
+        del back
+        here = [torch.empty(shape, dtype=dt, device="cuda") for dt in (torch.float16, torch.float32) for _ in range(4)]
+        assert all(x.data_ptr() != where for x in here)
+    torch.cuda.synchronize()
+    pool.check()
+    pool.release()
+
+
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
 def test_a_serving_run(cuda_device, code):
     """Prompt, decode steps and drafts with a roll-back, together as an engine uses them: q and K rotated, K and V written
