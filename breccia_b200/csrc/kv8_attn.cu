@@ -23,7 +23,8 @@
 //     their own may overlap.
 //
 // Two reference exponents per row, near the running maxima: m of the scores s (for the sum of probabilities), and M of
-// s + e_v, the exponent at which a cell's V codes enter the result.  Weights are 2^(s + e_v - M + 7), below 2^15 even when a
+// s + e_v, the exponent at which a cell's V codes enter the result, kept as M - m (a difference of two large scores is exact,
+// what is added to one is lost).  Weights are 2^(s + e_v - M + 7), below 2^15 even when a
 // score lies 2^8 over its reference, so binary16 keeps cells down to 2^-31 of the heaviest one, and a page whose V scale
 // dwarfs the others' neither overflows nor silences them.
 #include <algorithm>
@@ -39,7 +40,7 @@ constexpr uint32_t MIN_SHARE = 4;        // page-units a CTA takes at least
 constexpr uint32_t SMEM_LIMIT = 232448;  // 227 KiB
 constexpr uint32_t MAX_STAGES = 48;
 constexpr float HEADROOM = 8.f, WEIGHT_SHIFT = 7.f;   // a weight is at most 2^(WEIGHT_SHIFT + HEADROOM), half of binary16's greatest
-constexpr float NONE = -1e30f;           // running maximum before any cell
+constexpr float NONE = -3e38f;           // running maximum before any cell
 
 struct AttnParams {
     const void *q;
@@ -48,7 +49,7 @@ struct AttnParams {
     const uint32_t *block_tables, *seq_lens, *cu_q;
     const uint8_t *k_layer, *v_layer;
     uint32_t *prefix;        // workspace: cost of the sequences before each
-    float *ml;               // [slot][row of a unit][m, M, l, -]
+    float *ml;               // [slot][row of a unit][m, M - m, l, -]
     float *acc;              // [slot][row of a unit][head_dim]
     uint32_t *status;
     uint64_t page_bytes;
@@ -75,7 +76,7 @@ __host__ __device__ inline Smem smem_layout(uint32_t hd, uint32_t warps, uint32_
     if (prec) at += q_bufs * s.q_bytes;
     s.scratch = at;                       // [warp][row of a tile][head_dim + one 16-byte group]
     at += warps * 8u * (hd + 4u) * 4u;
-    s.stat = at;                          // [warp][row of two tiles][m, M, l, -]
+    s.stat = at;                          // [warp][row of two tiles][m, M - m, l, -]
     at += warps * 16u * 16u;
     s.row_fac = at;                       // [buffer][head][row]
     at += q_bufs * kvb * pass_rows * 4u;
@@ -519,38 +520,46 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
 
             // ---- softmax against the rows' reference exponents; weights to B fragments [cells][rows].  The references
             // move only when a score passes one by more than 2^HEADROOM, so an ordinary page needs no maximum across the warp.
+            // The weights' reference is kept relative to the scores' one, and scores enter as differences from that: small
+            // numbers beside a large score would be lost.  (The fused difference sees the unrounded score; where its rounding alone passes
+            // the reference by 2^HEADROOM, beyond 2^27, the branch takes the rounded one.)
             const bool good = ks > 0.f;
             const bool edge = cell0 + 16u > vis_min || !good;
             uint32_t pw[RT][2], pw_lo[RT][2];
 #pragma unroll
             for (int n = 0; n < RT; ++n) {
-                float wt[4];
+                float df[4], wt[4];   // scores less their reference, weights
                 bool over = false;
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {   // the thread's two rows: cells gr and gr + 8
                     const float kf = fac[n][x] * ks;
-                    s[n][x] *= kf;
-                    s[n][x + 2] *= kf;
+                    df[x] = fmaf(s[n][x], kf, -m_run[n][x]);
+                    df[x + 2] = fmaf(s[n][x + 2], kf, -m_run[n][x]);
                     if (edge) {
                         keep_branch();
-                        if (!good || cell0 + gr >= vis[n][x]) s[n][x] = -INFINITY;
-                        if (!good || cell0 + gr + 8u >= vis[n][x]) s[n][x + 2] = -INFINITY;
+                        if (!good || cell0 + gr >= vis[n][x]) df[x] = -INFINITY;
+                        if (!good || cell0 + gr + 8u >= vis[n][x]) df[x + 2] = -INFINITY;
                     }
-                    over |= fmaxf(s[n][x], s[n][x + 2]) > fminf(m_run[n][x], w_run[n][x] - ev) + HEADROOM;
+                    over |= fmaxf(df[x], df[x + 2]) > fminf(0.f, w_run[n][x] - ev) + HEADROOM;
                 }
                 if (__any_sync(0xffffffffu, over)) {
                     float f[2];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        float top = fmaxf(s[n][x], s[n][x + 2]);
+                        const float kf = fac[n][x] * ks;
+                        const float s0 = df[x] == -INFINITY ? df[x] : s[n][x] * kf, s1 = df[x + 2] == -INFINITY ? df[x + 2] : s[n][x + 2] * kf;
+                        float top = fmaxf(s0, s1);
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                        const float m_new = fmaxf(m_run[n][x], top), w_new = fmaxf(w_run[n][x], top + ev);
-                        l_run[n][x] *= brc::fast_exp2(m_run[n][x] - m_new);
-                        f[x] = brc::fast_exp2(w_run[n][x] - w_new);
+                        const float m_new = fmaxf(m_run[n][x], top), by = m_run[n][x] - m_new;
+                        const float w_old = w_run[n][x] + by, w_new = fmaxf(w_old, top - m_new + ev);
+                        l_run[n][x] *= brc::fast_exp2(by);
+                        f[x] = brc::fast_exp2(w_old - w_new);
                         m_run[n][x] = m_new;
                         w_run[n][x] = w_new;
+                        df[x] = s0 - m_new;
+                        df[x + 2] = s1 - m_new;
                     }
 #pragma unroll
                     for (int j = 0; j < (int)SLABS * 8; ++j) {
@@ -563,9 +572,9 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const float shift = ev - w_run[n][x] + WEIGHT_SHIFT;
-                    l_run[n][x] += brc::fast_exp2(s[n][x] - m_run[n][x]) + brc::fast_exp2(s[n][x + 2] - m_run[n][x]);
-                    wt[x] = brc::fast_exp2(s[n][x] + shift);
-                    wt[x + 2] = brc::fast_exp2(s[n][x + 2] + shift);
+                    l_run[n][x] += brc::fast_exp2(df[x]) + brc::fast_exp2(df[x + 2]);
+                    wt[x] = brc::fast_exp2(df[x] + shift);
+                    wt[x + 2] = brc::fast_exp2(df[x + 2] + shift);
                 }
                 const uint32_t a = brc::pack_half2(wt[0], wt[1]), b = brc::pack_half2(wt[2], wt[3]);
                 pw[n][0] = brc::movmatrix_trans(a);
@@ -660,12 +669,15 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
 #pragma unroll
                 for (uint32_t q = 0; q < LANES; ++q) {
                     m = fmaxf(m, st[q * STEP * 16u].x);
-                    wm = fmaxf(wm, st[q * STEP * 16u].y);
                 }
 #pragma unroll
-                for (uint32_t q = 0; q < LANES; ++q) l += st[q * STEP * 16u].z * brc::fast_exp2(st[q * STEP * 16u].x - m);
-                f[x] = brc::fast_exp2(w_run[n][x] - wm);
-                if (whole) f[x] *= l == 0.f ? 0.f : brc::fast_exp2(wm - m - WEIGHT_SHIFT) / l;
+                for (uint32_t q = 0; q < LANES; ++q) {
+                    const float by = st[q * STEP * 16u].x - m;
+                    wm = fmaxf(wm, st[q * STEP * 16u].y + by);
+                    l += st[q * STEP * 16u].z * brc::fast_exp2(by);
+                }
+                f[x] = brc::fast_exp2(w_run[n][x] + (m_run[n][x] - m) - wm);
+                if (whole) f[x] *= l == 0.f ? 0.f : brc::fast_exp2(wm - WEIGHT_SHIFT) / l;
                 else if (pl == 0 && gr == 0)
                     *reinterpret_cast<float4 *>(p.ml + (slot + hk * PASS + (rg * RT + n) * 8u + 2u * t + x) * 4u) = make_float4(m, wm, l, 0.f);
             }
@@ -719,6 +731,14 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
     if (!ok && lane == 0) { atomicOr(p.status, BRC_DEV_WAIT_LIMIT); p.status[1] = blockIdx.x; }
 }
 
+// A load under a predicate, for rows of many partials: left to the compiler they become branches, and each load waits for the one in
+// front of it (the merge of 131 072 cells: 8.6 us, 6.8 so; the few partials of a batch's rows are better off with the branch: a
+// call of 33.0 us, 33.7 so).
+__device__ __forceinline__ void load_if(bool live, const float *at, float4 &v) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t@p ld.global.v4.f32 {%0,%1,%2,%3}, [%5];\n\t}"
+                 : "+f"(v.x), "+f"(v.y), "+f"(v.z), "+f"(v.w) : "r"((uint32_t)live), "l"(at) : "memory");
+}
+
 // The partials that the shares' boundaries left of each (unit, query row), merged in share order; zeros for a sequence without
 // cells.  Units that one share covered are finished already.  W warps per row, ROWS rows per CTA, B partials of a warp
 // in flight (their sums and exponents together: one round trip).
@@ -749,29 +769,34 @@ __global__ void __launch_bounds__(W * ROWS * 32) kv8_merge_kernel(const AttnPara
 #pragma unroll
         for (uint32_t q = 0; q < B; ++q) {
             const uint32_t i = i0 + W * q;
+            const uint64_t a = (uint64_t)((2u * (c0 + i) + (i == 0 ? 1u : 0u)) * p.kvb + h) * p.pass_rows + r;
             st[q] = make_float4(NONE, NONE, 0.f, 0.f);
 #pragma unroll
             for (uint32_t j = 0; j < PER / 4; ++j) x[q][j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (i < n) {
-                const uint64_t a = (uint64_t)((2u * (c0 + i) + (i == 0 ? 1u : 0u)) * p.kvb + h) * p.pass_rows + r;
+            if (W > 1) {
+                load_if(i < n, p.ml + a * 4u, st[q]);
+#pragma unroll
+                for (uint32_t j = 0; j < PER / 4; ++j) load_if(i < n, p.acc + a * HD + lane * 4u + 128u * j, x[q][j]);
+            } else if (i < n) {
                 st[q] = *reinterpret_cast<const float4 *>(p.ml + a * 4u);
 #pragma unroll
                 for (uint32_t j = 0; j < PER / 4; ++j) x[q][j] = *reinterpret_cast<const float4 *>(p.acc + a * HD + lane * 4u + 128u * j);
             }
         }
-        float m_new = m, w_new = wm;
+        float m_new = m;
 #pragma unroll
-        for (uint32_t q = 0; q < B; ++q) {
-            m_new = fmaxf(m_new, st[q].x);
-            w_new = fmaxf(w_new, st[q].y);
-        }
-        const float f = brc::fast_exp2(wm - w_new);
+        for (uint32_t q = 0; q < B; ++q) m_new = fmaxf(m_new, st[q].x);
+        const float w_old = wm + (m - m_new);   // relative to the new maximum, as w_new
+        float w_new = w_old;
+#pragma unroll
+        for (uint32_t q = 0; q < B; ++q) w_new = fmaxf(w_new, st[q].y + (st[q].x - m_new));
+        const float f = brc::fast_exp2(w_old - w_new);
         l *= brc::fast_exp2(m - m_new);
 #pragma unroll
         for (uint32_t j = 0; j < PER; ++j) v[j] *= f;
 #pragma unroll
         for (uint32_t q = 0; q < B; ++q) {
-            const float g = brc::fast_exp2(st[q].y - w_new);
+            const float g = brc::fast_exp2(st[q].y + (st[q].x - m_new) - w_new);
             l += st[q].z * brc::fast_exp2(st[q].x - m_new);
 #pragma unroll
             for (uint32_t j = 0; j < PER / 4; ++j) {
@@ -787,7 +812,7 @@ __global__ void __launch_bounds__(W * ROWS * 32) kv8_merge_kernel(const AttnPara
     const uint64_t tok0 = p.cu_q ? p.cu_q[s] : (uint64_t)s * p.max_q;
     const uint64_t head_row = (tok0 + gr_row / p.group) * p.n_head + (hg * p.kvb + h) * p.group + gr_row % p.group;
     if constexpr (W == 1) {
-        const float f = l == 0.f ? 0.f : brc::fast_exp2(wm - m - WEIGHT_SHIFT) / l;
+        const float f = l == 0.f ? 0.f : brc::fast_exp2(wm - WEIGHT_SHIFT) / l;
 #pragma unroll
         for (uint32_t j = 0; j < PER; j += 4) {
             float x[4] = {v[j] * f, v[j + 1] * f, v[j + 2] * f, v[j + 3] * f};
@@ -804,19 +829,18 @@ __global__ void __launch_bounds__(W * ROWS * 32) kv8_merge_kernel(const AttnPara
         m = wm = NONE;
         l = 0.f;
 #pragma unroll
-        for (uint32_t w = 0; w < W; ++w) {
-            m = fmaxf(m, warp_stat[w].x);
-            wm = fmaxf(wm, warp_stat[w].y);
-        }
+        for (uint32_t w = 0; w < W; ++w) m = fmaxf(m, warp_stat[w].x);
+#pragma unroll
+        for (uint32_t w = 0; w < W; ++w) wm = fmaxf(wm, warp_stat[w].y + (warp_stat[w].x - m));
 #pragma unroll
         for (uint32_t w = 0; w < W; ++w) {
             const float4 st = warp_stat[w];
-            const float g = brc::fast_exp2(st.y - wm);
+            const float g = brc::fast_exp2(st.y + (st.x - m) - wm);
             l += st.z * brc::fast_exp2(st.x - m);
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] += part[w][d + e] * g;
         }
-        const float f = l == 0.f ? 0.f : brc::fast_exp2(wm - m - WEIGHT_SHIFT) / l;
+        const float f = l == 0.f ? 0.f : brc::fast_exp2(wm - WEIGHT_SHIFT) / l;
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] *= f;
         finish_row(p, HD, head_row, d, x);

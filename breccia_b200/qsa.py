@@ -642,8 +642,8 @@ def kv8_attend(pool: KvPool, layer: int, q: torch.Tensor, block_tables: torch.Te
                out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None, gate: torch.Tensor | None = None,
                gate_head_stride: int = 0, stream=None) -> torch.Tensor:
     """Attention over an 8-bit pool for the last T tokens of each sequence (brc_kv8_attn): q [tokens, n_head, hd], T = max_q, or
-    ragged by cu_q [n_seqs + 1] int32 with T <= max_q; token i of T sees seq_lens[s] - (T - 1 - i) cells.  `workspace` from
-    kv8_workspace; calls that may run at the same time need one each."""
+    ragged by cu_q [n_seqs + 1] int32 with T <= max_q; token i of T sees seq_lens[s] - (T - 1 - i) cells.  `out` may be q.
+    `workspace` from kv8_workspace; calls that may run at the same time need one each."""
     device = pool.device
     n_seqs, stride = block_tables.shape
     if q.dim() != 3 or q.shape[2] != pool.head_dim or not q.is_contiguous() or q.get_device() != device:
@@ -659,6 +659,13 @@ def kv8_attend(pool: KvPool, layer: int, q: torch.Tensor, block_tables: torch.Te
         out = _new(stream, lambda: torch.empty_like(q, dtype=out_dtype))
     elif out.shape != q.shape or not out.is_contiguous() or out.get_device() != device:
         raise BrcError(_lib.ERR_INVALID, f"kv8_attend: out {tuple(out.shape)} on {out.device} beside q {tuple(q.shape)}")
+    elif out.data_ptr() < q.data_ptr() + q.nbytes and q.data_ptr() < out.data_ptr() + out.nbytes and \
+            not (out.data_ptr() == q.data_ptr() and out.dtype == q.dtype):
+        raise BrcError(_lib.ERR_INVALID, "kv8_attend: out overlaps q without being the same rows")
+    if gate is not None and gate.numel() and tokens:
+        has = 1 + sum((n - 1) * s for n, s in zip(gate.shape, gate.stride()))
+        if has < (tokens * n_head - 1) * gate_head_stride + hd:
+            raise BrcError(_lib.ERR_INVALID, f"kv8_attend: gate {tuple(gate.shape)} with strides {gate.stride()} for {tokens * n_head} rows of {hd} every {gate_head_stride} values")
     if workspace.get_device() != device or (gate is not None and (gate.get_device() != device or gate.dtype != torch.float32)):
         raise BrcError(_lib.ERR_INVALID, f"kv8_attend: workspace on {workspace.device}, gate {None if gate is None else (gate.dtype, gate.device)}: "
                                          f"cuda:{device} and float32 wanted")

@@ -373,7 +373,8 @@ BRC_API brc_status brc_kv8_read(brc_pool *pool, uint32_t layer, const uint32_t *
  * over the cells c < seq_lens[s] - (T - 1 - i), kv head = h * n_kv_head / n_head.
  * A row that sees no cell yields zeros.  Cells at or past seq_lens[s] never
  * reach a result.  q and out are packed [tokens][n_head][head_dim], f32, f16 or
- * bf16 each; gate as in brc_paged_decode_attn.  The dot products and the
+ * bf16 each; out may be q's own memory when the types agree, and overlaps it in
+ * no other way; gate as in brc_paged_decode_attn.  The dot products and the
  * softmax are carried in f32 over exact products of the codes; the
  * probabilities are rounded to binary16 when both q and out are 16-bit and kept
  * as two binary16 parts (22 bits) otherwise.  A row with an infinity or NaN in q yields NaN.

@@ -534,6 +534,51 @@ def test_two_streams_and_two_graphs_side_by_side(cuda_device):
     pool.release()
 
 
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+def test_out_in_place_of_q(cuda_device, dt):
+    """Whole units, cut ones, several passes of rows, a sequence without cells: the same bits as beside q."""
+    lens = [5000, 0, 33, 700]
+    tables, n_pages = scattered(5, lens)
+    pool = KvPool(0, 1, 2, 128, n_pages, kv8="e4m3")
+    fill(pool, 21)
+    t, n = dev(tables), dev(lens)
+    for n_head, max_q in ((8, 1), (16, 9)):   # 4 rows a unit; 72: three passes
+        q = torch.randn(4 * max_q, n_head, 128, device="cuda").to(DTYPES[dt])
+        ws = kv8_workspace(pool, 4, n_head, max_q)
+        want = kv8_attend(pool, 0, q, t, n, 5000, ws, max_q=max_q)
+        assert kv8_attend(pool, 0, q, t, n, 5000, ws, max_q=max_q, out=q) is q
+        assert torch.equal(q, want)
+    with pytest.raises(BrcError):
+        wide = torch.zeros(5, 8, 128, device="cuda")
+        kv8_attend(pool, 0, wide[:4], t, n, 5000, kv8_workspace(pool, 4, 8), out=wide[1:])
+    for gate, stride in ((torch.ones(4 * 8 * 128 - 1, device="cuda"), 128), (torch.ones(4, 8, 128, device="cuda"), 256)):
+        with pytest.raises(BrcError):
+            kv8_attend(pool, 0, wide[:4], t, n, 5000, kv8_workspace(pool, 4, 8), gate=gate, gate_head_stride=stride)
+    pool.check()
+    pool.release()
+
+
+def test_scores_of_any_size(cuda_device):
+    """Scores near either end of f32, all cells alike: their mean, whatever the score.  (The sums are exact up to f32 roundings of 40 equal
+    weights; a weight is exactly 2^7.)"""
+    pool = KvPool(0, 1, 2, 128, 3, kv8="int8")
+    t, n = dev([[0, 1, 2]]), dev([40])
+    k = torch.full((40, 2, 128), 2.0 ** 60, device="cuda")
+    v = torch.randint(-100, 100, (40, 2, 128), device="cuda").float()
+    v[:, :, 0] = 100.0   # the scale: 1 in every page
+    kv8_append(pool, 0, k, v, t, dev([0]), 40, 40)
+    want = v.double().mean(0)
+    ws = kv8_workspace(pool, 1, 2)
+    for size in (0.0, 2.0 ** -100, 2.0 ** 20, 2.0 ** 50, 2.0 ** 59):   # q . k up to 2^126
+        for sign in (1.0, -1.0):
+            q = torch.full((1, 2, 128), sign * size, device="cuda")
+            out = kv8_attend(pool, 0, q, t, n, 40, ws, scale=1.0)
+            # 40 additions on either side of the division and three more roundings, of sums of |v| <= 100
+            assert (out[0].double() - want).abs().max() <= 100 * 83 * 2.0 ** -24, (size, sign)
+    pool.check()
+    pool.release()
+
+
 def test_outputs_belong_to_the_stream_that_writes_them(cuda_device):
     """An output made for a call on another stream must not come from memory that the current stream may still use."""
     pool = KvPool(0, 1, 2, 128, 4, kv8="int8")
