@@ -623,8 +623,10 @@ def kv8_read(pool: KvPool, layer: int, block_tables: torch.Tensor, pos0: torch.T
     tables, at = _words(block_tables, device, "kv8_read: block_tables"), _words(pos0, device, "kv8_read: pos0", n_seqs)
     cu = None if cu_tokens is None else _words(cu_tokens, device, "kv8_read: cu_tokens", n_seqs + 1)
     code = _dtype(dtype, "kv8_read")
-    both = _new(stream, lambda: torch.empty((2, total_tokens, pool.n_kv_head, pool.head_dim), dtype=dtype, device=block_tables.device))
-    k, v = both[0], both[1]
+    n_kv, hd = pool.n_kv_head, pool.head_dim
+    # (two tensors by their strides take the host half as long as one and its two halves)
+    k, v = _new(stream, lambda: [torch.empty_strided((total_tokens, n_kv, hd), (n_kv * hd, hd, 1), dtype=dtype, device=block_tables.device)
+                                 for _ in range(2)])
     _lib.check(_lib.load().brc_kv8_read(pool.handle, layer, tables, stride, at, n_seqs, tokens_per_seq, cu, total_tokens, max_pos_end, k.data_ptr(),
                                         v.data_ptr(), code, _raw_stream(stream, device)))
     return k, v
