@@ -16,9 +16,9 @@ DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 
 
 def tolerance(x, want, m, dtype):
-    """f32 arithmetic on the pair: cos and sin off by at most 4 units of 2^-24 (sincospif's two, the angle's own rounding, the
-    factor), two products and a sum of three roundings of 2^-24 of the terms: 8 * 2^-24 * (|x| + |y|) m; then the type's half
-    step, and below its normal range half its least spacing."""
+    """f32 arithmetic on the pair: cos and sin (times the factor, in 64 bits) rounded once, two products and a sum of three roundings
+    of 2^-24 of the terms: within 8 * 2^-24 * (|x| + |y|) m; then the type's half step, and below its normal range half its
+    least spacing."""
     fi = torch.finfo(dtype)
     pair = np.abs(x).max(-1, keepdims=True) * 2
     return 8 * 2.0 ** -24 * pair * m + (fi.eps / 2 * np.abs(want) if dtype != torch.float32 else 0) + fi.tiny * fi.eps
