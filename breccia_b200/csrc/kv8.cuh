@@ -113,35 +113,6 @@ template <> __device__ __forceinline__ float from_f32<0>(float x) { return x; }
 template <> __device__ __forceinline__ __half from_f32<1>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<2>(float x) { return __float2bfloat16_rn(x); }
 
-// Eight consecutive elements; `vec`: the address is a multiple of 16 bytes.
-template <int DT>
-__device__ __forceinline__ void load8(const typename elem<DT>::t *p, bool vec, float (&v)[8]) {
-    if (!vec) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32(p[i]);
-        return;
-    }
-    if constexpr (DT == 0) {
-        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        const uint4 u = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (DT == 1) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-                v[2 * i] = f.x;
-                v[2 * i + 1] = f.y;
-            } else {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
-        }
-    }
-}
-
 // The larger of a magnitude, given as bits, and |x|; NaN wins (the bits of one are above those of infinity).
 __device__ __forceinline__ uint32_t max_magnitude(uint32_t m, float x) {
     float r;
@@ -149,7 +120,8 @@ __device__ __forceinline__ uint32_t max_magnitude(uint32_t m, float x) {
     return __float_as_uint(r);
 }
 
-// Eight consecutive elements as they lie in memory: half the registers of their f32 values for the 16-bit types.
+// Eight consecutive elements as they lie in memory (`vec`: at a multiple of 16 bytes): half the registers of their f32 values for the
+// 16-bit types.
 template <int DT>
 struct raw8 {
     static constexpr int WORDS = DT == 0 ? 8 : 4;
@@ -218,21 +190,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     } else {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t *>(&h);
-    }
-}
-
-template <int DT>
-__device__ __forceinline__ void store8(typename elem<DT>::t *p, bool vec, const float (&v)[8]) {
-    if (!vec) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = from_f32<DT>(v[i]);
-        return;
-    }
-    if constexpr (DT == 0) {
-        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-        *reinterpret_cast<uint4 *>(p) = make_uint4(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7]));
     }
 }
 

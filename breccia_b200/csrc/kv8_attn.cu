@@ -17,7 +17,7 @@
 //     head_dim may run in any order, so K's columns are dealt out 16 bytes to a thread, and V's columns likewise become
 //     the output rows; the 128-byte swizzle of the TMA box keeps every such read free of bank conflicts;
 //   - all (sequence, kv-head group, pass) units form one list of page-units cut into equal shares, one persistent CTA per
-//     SM; one warp streams the pages with TMA into a ring, eight consume.  A unit cut by a share boundary leaves partial
+//     SM; one warp streams the pages with TMA into a ring, eight or twelve consume.  A unit cut by a share boundary leaves partial
 //     results in the caller's workspace, and a second kernel, launched with its prologue overlapped (programmatic
 //     dependent launch), merges them.  No counters and no flags: nothing survives a call, so calls with workspaces of
 //     their own may overlap.
@@ -133,10 +133,16 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
 __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 
 // One load of q rows in any of the three types: eight consecutive values of head row `r` from column d.
+template <int DT>
+__device__ __forceinline__ void load_q8_as(const AttnParams &p, uint64_t at, float (&v)[8]) {
+    brc::raw8<DT> r;
+    r.load(static_cast<const typename brc::elem<DT>::t *>(p.q) + at, true);
+    r.values(v);
+}
 __device__ __forceinline__ void load_q8(const AttnParams &p, uint64_t at, float (&v)[8]) {
-    if (p.q_dtype == 0) brc::load8<0>(static_cast<const float *>(p.q) + at, true, v);
-    else if (p.q_dtype == 1) brc::load8<1>(static_cast<const __half *>(p.q) + at, true, v);
-    else brc::load8<2>(static_cast<const __nv_bfloat16 *>(p.q) + at, true, v);
+    if (p.q_dtype == 0) load_q8_as<0>(p, at, v);
+    else if (p.q_dtype == 1) load_q8_as<1>(p, at, v);
+    else load_q8_as<2>(p, at, v);
 }
 
 // A share's walk over the units: [lo, hi) on the axis of costs, and where the unit in hand begins on it.
@@ -328,8 +334,9 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
     Segment g = start->seg;
     bool more = g.n != 0;
 
-    // Registers: launched with 168 / 128 / 96 a thread (8 / 12 / 16 consuming warps and four more), of which the four others
+    // Registers: launched with 168 / 128 a thread (8 / 12 consuming warps and four more), of which the four others
     // keep 56 and hand the rest to the consumers; the sums stay within what the block was launched with.
+    static_assert(W == 8 || W == 12, "");
     if (warp >= W) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         bool ok = true;
@@ -388,8 +395,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
         return;
     }
     if constexpr (W == 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    else if constexpr (W == 12) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
 
     // ---------------------------------------------------------------------- consumers
     const uint32_t t = lane & 3u, gr = lane >> 2;            // thread of a group, group
@@ -928,9 +934,9 @@ brc_status launch_rows(const brc_pool *pool, const AttnParams &p, uint32_t grid,
     // Warps: what the registers of the sums allow and the ring bears (a stage for each warp that takes pages in turn, twice
     // over).  Measured (us) at 8, 12, 16 warps of head_dim 128: 32 sequences, 8 kv heads 54.4, 51.4, 53.5; drafts of 24 sequences 50.4, 50.2,
     // 52.4; eight tokens each 79, 73, 84.
-    constexpr int W1 = HD == 128 ? 12 : 8, W2 = W1;
-    if (rt == 1) return launch<HD, CODE, PREC, 1, 1, KVB, W1>(pool, p, grid, merge_rows, st);
-    return p.row_groups == 1 ? launch<HD, CODE, PREC, 2, 1, KVB, W2>(pool, p, grid, merge_rows, st) : launch<HD, CODE, PREC, 2, 2, KVB, W2>(pool, p, grid, merge_rows, st);
+    constexpr int W = HD == 128 ? 12 : 8;
+    if (rt == 1) return launch<HD, CODE, PREC, 1, 1, KVB, W>(pool, p, grid, merge_rows, st);
+    return p.row_groups == 1 ? launch<HD, CODE, PREC, 2, 1, KVB, W>(pool, p, grid, merge_rows, st) : launch<HD, CODE, PREC, 2, 2, KVB, W>(pool, p, grid, merge_rows, st);
 }
 
 template <int HD, uint32_t CODE>

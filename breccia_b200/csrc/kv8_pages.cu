@@ -270,8 +270,10 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const PagesParams p) {
 #pragma unroll
                 for (uint32_t y = 0; y < 4; ++y) v[4 * x + y] = a[y] * s[u];
             }
-            if constexpr (N == 8) brc::store8<DT>(out + (uint64_t)at[u] * N, true, v);
-            else *reinterpret_cast<float4 *>(out + (uint64_t)at[u] * N) = make_float4(v[0], v[1], v[2], v[3]);
+            T *to = out + (uint64_t)at[u] * N;
+            if constexpr (N == 8)
+                *reinterpret_cast<uint4 *>(to) = make_uint4(brc::pack2<DT>(v[0], v[1]), brc::pack2<DT>(v[2], v[3]), brc::pack2<DT>(v[4], v[5]), brc::pack2<DT>(v[6], v[7]));
+            else *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
         }
     }
 }

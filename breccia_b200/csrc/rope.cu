@@ -64,7 +64,7 @@ enum Pairing { INTERLEAVED, HALF_CHUNKS, HALF_ANY };   // HALF_CHUNKS: n_rot / 2
 constexpr uint32_t ROPE_WARPS = 8, ROPE_MAX_PAIRS = 128, ROPE_STAGE = 256 + 8;   // staged values of a warp: 256, one word of shift every 32
 
 // Rows of HD values whose addresses are multiples of 16 bytes.  `splits` warps share a token's rows.  64 bytes a lane are turned
-// while the next 64 travel, three CTAs an SM: 16384 tokens of 40 x 128 bf16 in 55.1 us interleaved (6.1 TB/s), 56.6 half;
+// while the next 64 travel, three CTAs an SM: 16384 tokens of 40 x 128 bf16 in 54.9 us interleaved (6.1 TB/s), 56.2 half;
 // with 32 bytes a lane 58.0 and 59.7, with 16 and no look-ahead 58.3 and 74.9.
 template <int DT, int HD, int PAIR>
 __global__ void __launch_bounds__(ROPE_WARPS * 32, 3) rope_kernel(const RopeParams p) {
