@@ -26,7 +26,8 @@
 // s + e_v, the exponent at which a cell's V codes enter the result, kept as M - m (a difference of two large scores is exact,
 // what is added to one is lost).  Weights are 2^(s + e_v - M + 7), below 2^15 even when a
 // score lies 2^8 over its reference, so binary16 keeps cells down to 2^-31 of the heaviest one, and a page whose V scale
-// dwarfs the others' neither overflows nor silences them.
+// dwarfs the others' neither overflows nor silences them.  A weight goes to the tensor cores as two binary16 parts, 22 of its 24 bits,
+// whatever the types of q and out: one part's 2^-12 shows in a 16-bit result wherever values cancel.
 #include <algorithm>
 #include <atomic>
 
@@ -64,7 +65,7 @@ struct Smem {   // byte offsets behind the ring
     uint32_t stage_bytes, q, q_lo, q_bytes, scratch, stat, row_fac, row_vis, bars, sched, total;
 };
 
-__host__ __device__ inline Smem smem_layout(uint32_t hd, uint32_t warps, uint32_t kvb, uint32_t pass_rows, bool prec, uint32_t n_stages,
+__host__ __device__ inline Smem smem_layout(uint32_t hd, uint32_t warps, uint32_t kvb, uint32_t pass_rows, bool split_q, uint32_t n_stages,
                                             uint32_t q_bufs) {
     Smem s;
     s.stage_bytes = kvb * 2u * 16u * hd;
@@ -73,7 +74,7 @@ __host__ __device__ inline Smem smem_layout(uint32_t hd, uint32_t warps, uint32_
     s.q_bytes = kvb * pass_rows * hd * 2u;
     at += q_bufs * s.q_bytes;
     s.q_lo = at;
-    if (prec) at += q_bufs * s.q_bytes;
+    if (split_q) at += q_bufs * s.q_bytes;
     s.scratch = at;                       // [warp][row of a tile][head_dim + one 16-byte group]
     at += warps * 8u * (hd + 4u) * 4u;
     s.stat = at;                          // [warp][row of two tiles][m, M - m, l, -]
@@ -185,7 +186,7 @@ __device__ __forceinline__ bool next_segment(const AttnParams &p, Cursor &c, Seg
 // [8-row tile][pair of 16-column steps][lane][2 x 4 values]; column d belongs to step 8 (d / 128) + 4 (d / 16 % 2) +
 // d / 4 % 4 and thread d / 32 % 4 of its row's group.  A row takes HD / 8 lanes; warp `w` of `n_w` has every n_w-th set of
 // 256 / HD rows, U sets of loads in flight; `meanwhile` runs behind the first loads.
-template <int HD, bool PREC, int U, class F>
+template <int HD, bool SPLIT_Q, int U, class F>
 __device__ __forceinline__ void stage_q(const AttnParams &p, const Smem &L, uint8_t *smem, const Segment &g, uint32_t buf, uint32_t w,
                                         uint32_t n_w, uint32_t lane, F &&meanwhile) {
     constexpr uint32_t LANES = HD / 8, SET = 32 / LANES;
@@ -237,20 +238,21 @@ __device__ __forceinline__ void stage_q(const AttnParams &p, const Smem &L, uint
                 b[i] = brc::pack_half2(x - f.x, y - f.y);
             }
             *reinterpret_cast<uint4 *>(smem + L.q + at) = make_uint4(a[0], a[1], a[2], a[3]);
-            if (PREC) *reinterpret_cast<uint4 *>(smem + L.q_lo + at) = make_uint4(b[0], b[1], b[2], b[3]);
+            if (SPLIT_Q) *reinterpret_cast<uint4 *>(smem + L.q_lo + at) = make_uint4(b[0], b[1], b[2], b[3]);
         }
     }
 }
 
 // RT: tiles of eight query rows that a warp carries; RG: warps side by side on a page's rows; KVB: kv heads of a unit; W: consuming
-// warps.  PREC: q and the probabilities as two binary16 parts each.
-template <int HD, uint32_t CODE, bool PREC, int RT, int RG, int KVB, int W>
+// warps.  SPLIT_Q: q as two binary16 parts (f32 q; the 16-bit types are
+// exact in one).
+template <int HD, uint32_t CODE, bool SPLIT_Q, int RT, int RG, int KVB, int W>
 __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_constant__ CUtensorMap tm, const AttnParams p) {
     constexpr uint32_t SLABS = HD / 128, CONSUMERS = W * 32, ROW = HD + 4;
     constexpr uint32_t STEP = KVB * RG, LANES = W / STEP, PASS = RG * RT * 8, STAGE = KVB * 2 * 16 * HD, SLAB = STAGE / SLABS;   // LANES: warps that take pages in turn
     static_assert(W % STEP == 0 && CONSUMERS % (HD / 4) == 0, "");
     extern __shared__ __align__(1024) uint8_t smem[];
-    const Smem L = smem_layout(HD, W, KVB, PASS, PREC, p.n_stages, p.q_bufs);
+    const Smem L = smem_layout(HD, W, KVB, PASS, SPLIT_Q, p.n_stages, p.q_bufs);
     const uint32_t base = brc::smem_u32(smem);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t full0 = base + L.bars, empty0 = full0 + MAX_STAGES * 8u, q_full0 = empty0 + MAX_STAGES * 8u, q_empty0 = q_full0 + 16u;
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
                     const uint32_t buf = idx % p.q_bufs;
                     if (idx >= p.q_bufs) ok = brc::mbar_wait(q_empty0 + 8u * buf, (idx - p.q_bufs) / p.q_bufs & 1u);
                     if (!ok) break;
-                    stage_q<HD, PREC, 2>(p, L, smem, g, buf, warp - W - 1u, 3u, lane, [] {});
+                    stage_q<HD, SPLIT_Q, 2>(p, L, smem, g, buf, warp - W - 1u, 3u, lane, [] {});
                     __syncwarp();
                     if (lane == 0) brc::mbar_arrive(q_full0 + 8u * buf);
                 }
@@ -438,7 +440,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
         if (idx == 0) {   // the first unit's q: nobody has anything else to do yet
             // (scales asked for with the q rows: behind the first pages' boxes they would come 3 us later)
             bool asked = false;
-            stage_q<HD, PREC, RT == 1 ? 2 : 4>(p, L, smem, g, 0, warp, W, lane, [&] { scales_of(g, ids, ks_next, ev_next); asked = true; });
+            stage_q<HD, SPLIT_Q, RT == 1 ? 2 : 4>(p, L, smem, g, 0, warp, W, lane, [&] { scales_of(g, ids, ks_next, ev_next); asked = true; });
             if (!asked) scales_of(g, ids, ks_next, ev_next);
             brc::named_bar_sync(1, CONSUMERS);
         } else {
@@ -510,7 +512,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
                             const uint4 qf = lds128(smem, q_frag + n * 8u * HD * 2u + at);
                             mma(part[n][0], f0, qf.x, qf.y);
                             mma(part[n][1], f1, qf.z, qf.w);
-                            if (PREC) {
+                            if (SPLIT_Q) {
                                 const uint4 ql = lds128(smem, q_frag_lo + n * 8u * HD * 2u + at);
                                 mma(part[n][0], f0, ql.x, ql.y);
                                 mma(part[n][1], f1, ql.z, ql.w);
@@ -585,11 +587,9 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
                 const uint32_t a = brc::pack_half2(wt[0], wt[1]), b = brc::pack_half2(wt[2], wt[3]);
                 pw[n][0] = brc::movmatrix_trans(a);
                 pw[n][1] = brc::movmatrix_trans(b);
-                if (PREC) {
-                    const float2 ha = __half22float2(*reinterpret_cast<const __half2 *>(&a)), hb = __half22float2(*reinterpret_cast<const __half2 *>(&b));
-                    pw_lo[n][0] = brc::movmatrix_trans(brc::pack_half2(wt[0] - ha.x, wt[1] - ha.y));
-                    pw_lo[n][1] = brc::movmatrix_trans(brc::pack_half2(wt[2] - hb.x, wt[3] - hb.y));
-                }
+                const float2 ha = __half22float2(*reinterpret_cast<const __half2 *>(&a)), hb = __half22float2(*reinterpret_cast<const __half2 *>(&b));
+                pw_lo[n][0] = brc::movmatrix_trans(brc::pack_half2(wt[0] - ha.x, wt[1] - ha.y));
+                pw_lo[n][1] = brc::movmatrix_trans(brc::pack_half2(wt[2] - hb.x, wt[3] - hb.y));
             }
 
             // ---- O^T[head_dim][8 rows] += V^T P.  Output row gr of tile j is column 16 gr + j, row gr + 8 column 16 gr + 8 + j.
@@ -634,7 +634,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
 #pragma unroll
                         for (int n = 0; n < RT; ++n) {
                             mma(o[n][sl * 8u + 4u * y + j], fa[j], pw[n][0], pw[n][1]);
-                            if (PREC) mma(o[n][sl * 8u + 4u * y + j], fa[j], pw_lo[n][0], pw_lo[n][1]);
+                            mma(o[n][sl * 8u + 4u * y + j], fa[j], pw_lo[n][0], pw_lo[n][1]);
                         }
                 }
             }
@@ -881,20 +881,20 @@ Shape shape_of(const brc_pool *pool, uint32_t n_seqs, uint32_t n_head, uint32_t 
     return s;
 }
 
-template <int HD, uint32_t CODE, bool PREC, int RT, int RG, int KVB, int W>
+template <int HD, uint32_t CODE, bool SPLIT_Q, int RT, int RG, int KVB, int W>
 brc_status launch(const brc_pool *pool, AttnParams p, uint32_t grid, uint32_t merge_rows, cudaStream_t st) {
-    auto kern = kv8_attn_kernel<HD, CODE, PREC, RT, RG, KVB, W>;
+    auto kern = kv8_attn_kernel<HD, CODE, SPLIT_Q, RT, RG, KVB, W>;
     const uint32_t turns = W / (KVB * RG);
     // Ring depth: what fits, in multiples of the warps that take pages in turn, so that a stage is always consumed by the same
     // warps (a parity wait is only valid for a warp that knows the previous round of the barrier is over).
     auto depth = [&](uint32_t q_bufs) {
         uint32_t n = MAX_STAGES / turns * turns;
-        while (n > turns && smem_layout(HD, W, p.kvb, p.pass_rows, PREC, n, q_bufs).total > SMEM_LIMIT) n -= turns;
+        while (n > turns && smem_layout(HD, W, p.kvb, p.pass_rows, SPLIT_Q, n, q_bufs).total > SMEM_LIMIT) n -= turns;
         return n;
     };
     p.q_bufs = depth(2) == depth(1) ? 2u : 1u;   // the next unit's q is staged ahead where that costs no ring stage
     p.n_stages = depth(p.q_bufs);
-    const uint32_t smem = smem_layout(HD, W, p.kvb, p.pass_rows, PREC, p.n_stages, p.q_bufs).total;
+    const uint32_t smem = smem_layout(HD, W, p.kvb, p.pass_rows, SPLIT_Q, p.n_stages, p.q_bufs).total;
     if (smem > SMEM_LIMIT) return brc_fail(BRC_ERR_UNSUPPORTED, "8-bit attention: %u bytes of shared memory", smem);
     static std::atomic<uint64_t> ready{0};   // devices on which this kernel may use all shared memory
     const uint64_t bit = 1ull << (pool->device & 63);
@@ -929,20 +929,20 @@ brc_status launch(const brc_pool *pool, AttnParams p, uint32_t grid, uint32_t me
     return BRC_OK;
 }
 
-template <int HD, uint32_t CODE, bool PREC, int KVB>
+template <int HD, uint32_t CODE, bool SPLIT_Q, int KVB>
 brc_status launch_rows(const brc_pool *pool, const AttnParams &p, uint32_t grid, uint32_t rt, uint32_t merge_rows, cudaStream_t st) {
     // Warps: what the registers of the sums allow and the ring bears (a stage for each warp that takes pages in turn, twice
     // over).  Measured (us) at 8, 12, 16 warps of head_dim 128: 32 sequences, 8 kv heads 54.4, 51.4, 53.5; drafts of 24 sequences 50.4, 50.2,
     // 52.4; eight tokens each 79, 73, 84.
     constexpr int W = HD == 128 ? 12 : 8;
-    if (rt == 1) return launch<HD, CODE, PREC, 1, 1, KVB, W>(pool, p, grid, merge_rows, st);
-    return p.row_groups == 1 ? launch<HD, CODE, PREC, 2, 1, KVB, W>(pool, p, grid, merge_rows, st) : launch<HD, CODE, PREC, 2, 2, KVB, W>(pool, p, grid, merge_rows, st);
+    if (rt == 1) return launch<HD, CODE, SPLIT_Q, 1, 1, KVB, W>(pool, p, grid, merge_rows, st);
+    return p.row_groups == 1 ? launch<HD, CODE, SPLIT_Q, 2, 1, KVB, W>(pool, p, grid, merge_rows, st) : launch<HD, CODE, SPLIT_Q, 2, 2, KVB, W>(pool, p, grid, merge_rows, st);
 }
 
 template <int HD, uint32_t CODE>
-brc_status launch_kind(const brc_pool *pool, const AttnParams &p, uint32_t grid, bool prec, uint32_t rt, uint32_t merge_rows, cudaStream_t st) {
-    if (p.kvb == 2) return prec ? launch_rows<HD, CODE, true, 2>(pool, p, grid, rt, merge_rows, st) : launch_rows<HD, CODE, false, 2>(pool, p, grid, rt, merge_rows, st);
-    return prec ? launch_rows<HD, CODE, true, 1>(pool, p, grid, rt, merge_rows, st) : launch_rows<HD, CODE, false, 1>(pool, p, grid, rt, merge_rows, st);
+brc_status launch_kind(const brc_pool *pool, const AttnParams &p, uint32_t grid, bool split_q, uint32_t rt, uint32_t merge_rows, cudaStream_t st) {
+    if (p.kvb == 2) return split_q ? launch_rows<HD, CODE, true, 2>(pool, p, grid, rt, merge_rows, st) : launch_rows<HD, CODE, false, 2>(pool, p, grid, rt, merge_rows, st);
+    return split_q ? launch_rows<HD, CODE, true, 1>(pool, p, grid, rt, merge_rows, st) : launch_rows<HD, CODE, false, 1>(pool, p, grid, rt, merge_rows, st);
 }
 
 bool known_dtype(int32_t d) { return d == BRC_DTYPE_F32 || d == BRC_DTYPE_F16 || d == BRC_DTYPE_BF16; }
@@ -1030,17 +1030,17 @@ brc_status brc_kv8_attend(brc_pool *pool, const char *who, const brc_kv8_attn_ar
         return brc_fail(BRC_ERR_UNSUPPORTED, "%s: %u sequences of up to %u cells in %u passes each are too much for one call", who, a.n_seqs, a.max_seq_len,
                         s.units_per_seq);
     const uint32_t grid = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>(pool->sm_count, (most + MIN_SHARE - 1u) / MIN_SHARE));
-    const bool prec = a.q_dtype == BRC_DTYPE_F32 || a.out_dtype == BRC_DTYPE_F32;
+    const bool split_q = a.q_dtype == BRC_DTYPE_F32;
     const uint32_t merge_rows = s.kvb * s.pass_rows;
     cudaStream_t st = brc_stream(stream);
     brc_stage_begin(pool, BRC_STAGE_ATTN_PARTIAL, st);
     brc_status rc;
     if (pool->head_dim == 256)
-        rc = pool->kv8 == brc::KV8_E4M3 ? launch_kind<256, brc::KV8_E4M3>(pool, p, grid, prec, s.rt, merge_rows, st)
-                                        : launch_kind<256, brc::KV8_INT8>(pool, p, grid, prec, s.rt, merge_rows, st);
+        rc = pool->kv8 == brc::KV8_E4M3 ? launch_kind<256, brc::KV8_E4M3>(pool, p, grid, split_q, s.rt, merge_rows, st)
+                                        : launch_kind<256, brc::KV8_INT8>(pool, p, grid, split_q, s.rt, merge_rows, st);
     else
-        rc = pool->kv8 == brc::KV8_E4M3 ? launch_kind<128, brc::KV8_E4M3>(pool, p, grid, prec, s.rt, merge_rows, st)
-                                        : launch_kind<128, brc::KV8_INT8>(pool, p, grid, prec, s.rt, merge_rows, st);
+        rc = pool->kv8 == brc::KV8_E4M3 ? launch_kind<128, brc::KV8_E4M3>(pool, p, grid, split_q, s.rt, merge_rows, st)
+                                        : launch_kind<128, brc::KV8_INT8>(pool, p, grid, split_q, s.rt, merge_rows, st);
     brc_stage_end(pool, BRC_STAGE_ATTN_PARTIAL, st);
     return rc;
 }

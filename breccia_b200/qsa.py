@@ -644,7 +644,8 @@ def kv8_attend(pool: KvPool, layer: int, q: torch.Tensor, block_tables: torch.Te
                out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None, gate: torch.Tensor | None = None,
                gate_head_stride: int = 0, stream=None) -> torch.Tensor:
     """Attention over an 8-bit pool for the last T tokens of each sequence (brc_kv8_attn): q [tokens, n_head, hd], T = max_q, or
-    ragged by cu_q [n_seqs + 1] int32 with T <= max_q; token i of T sees seq_lens[s] - (T - 1 - i) cells.  `out` may be q.
+    ragged by cu_q [n_seqs + 1] int32 with T <= max_q; token i of T sees seq_lens[s] - (T - 1 - i) cells.  Sums and softmax
+    in f32, probabilities to 22 bits, one rounding to `out_dtype` (q's type unless given).  `out` may be q.
     `workspace` from kv8_workspace; calls that may run at the same time need one each."""
     device = pool.device
     n_seqs, stride = block_tables.shape

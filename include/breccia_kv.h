@@ -376,9 +376,9 @@ BRC_API brc_status brc_kv8_read(brc_pool *pool, uint32_t layer, const uint32_t *
  * bf16 each; out may be q's own memory when the types agree, and overlaps it in
  * no other way; gate as in brc_paged_decode_attn.  The dot products and the
  * softmax are carried in f32 over exact products of the codes; the
- * probabilities are rounded to binary16 when both q and out are 16-bit and kept
- * as two binary16 parts (22 bits) otherwise, those under 2^-31 of a row's largest
- * (each times its page's V scale) lost.  A row with an infinity or NaN in q yields NaN.
+ * probabilities, and q where it is f32, are kept as two binary16 parts (22 bits)
+ * for the products, probabilities under 2^-31 of a row's largest (each times its
+ * page's V scale) lost.  A row with an infinity or NaN in q yields NaN.
  * Up to 32 rows (T x heads per kv head) share one stream of the cache; more are
  * taken in passes of 32, each streaming it again: made for decode and drafts,
  * not for long prompts.

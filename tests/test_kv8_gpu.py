@@ -727,3 +727,34 @@ def test_pages_travel_with_their_scales(cuda_device, tmp_path):
         _lib.call("brc_tier_destroy", x)
     pool.release()
     other.release()
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("n_head,n_kv,hd,max_q", [(16, 2, 256, 1), (6, 3, 128, 1), (16, 2, 256, 2), (8, 2, 128, 9)])
+def test_sixteen_bit_results_are_rounded_once(cuda_device, code, dt, n_head, n_kv, hd, max_q):
+    """16-bit q and out: the result is the f32 one rounded to the type, its weights not rounded to 16 bits in front of that.
+
+    Scores near one another (q small), so that the exponent's own error is small and weights lie just under a power of two, where a
+    weight in one binary16 part would be off by up to 2^-12 of itself; two parts: 2^-22.  Few cells, and columns where values cancel."""
+    lens = [2, 3, 5, 9, 16, 17, 40, 300]
+    tables, n_pages = scattered(2, lens)
+    pool = KvPool(0, 1, n_kv, hd, n_pages, kv8=code)
+    values = fill(pool, 3)
+    q = (torch.randn(len(lens) * max_q, n_head, hd, device="cuda", generator=torch.Generator(device="cuda").manual_seed(4)) * 0.05).to(DTYPES[dt])
+    got = kv8_attend(pool, 0, q, dev(tables), dev(lens), max(lens), kv8_workspace(pool, len(lens), n_head, max_q), max_q=max_q)
+    pool.check()
+    assert got.dtype == DTYPES[dt]
+    got, qn, fi = got.double().cpu().numpy(), q.double().cpu().numpy(), torch.finfo(DTYPES[dt])
+    for s, n in enumerate(lens):
+        k, v = (cells(x, tables[s], n) for x in values)
+        for i in range(max_q):
+            want, mag, dot = ref.attention(qn[s * max_q + i], k, v, n - (max_q - 1 - i), 1 / math.sqrt(hd))
+            # as in run_and_compare with the two parts' 2^-22 on numerator and denominator; below the second part's range half binary16's
+            # least spacing, 2^-25 beside a heaviest weight of 2^7 or more, for each cell; then out's half step
+            exponent = 2 * (hd / 16 + 4) * 2.0 ** -22 * dot[:, None] + 4 * 2.0 ** -21
+            tol = mag * (2.0 ** -21 + 2 * exponent + 2 * (n / 16 + 32) * 2.0 ** -22) + n * 2.0 ** -32 * np.abs(v).max()
+            tol = tol * (1 + fi.eps) + fi.eps / 2 * np.abs(want) + fi.tiny * fi.eps
+            err = np.abs(got[s * max_q + i] - want)
+            assert (err <= tol).all(), (s, i, float((err - tol).max()), float(err.max()))
+    pool.release()
