@@ -148,6 +148,7 @@ SIGNATURES = {
     "brc_kv8_read": [_vp, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _u32, _vp, _vp, _i32, _vp],
     "brc_kv8_attn_workspace_bytes": [_vp, _u32, _u32, _u32, _u64p],
     "brc_kv8_attn": [_vp, _u32, _vp, _i32, _u32, _vp, _u32, _vp, _u32, _vp, _vp, _u32, _u32, _u32, _f32, _vp, _i32, _vp, _u64, _vp],
+    "brc_kv8_attn_ragged": [_vp, _u32, _vp, _i32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _vp, _u32, _u32, _u32, _f32, _vp, _i32, _vp, _u64, _vp],
     "brc_rope_freqs": [C.POINTER(RopeParams), _u64p, C.POINTER(C.c_double)],
     "brc_rope_apply": [_i32, _vp, _vp, _u32, _u64, _u64, _vp, _vp, _u32, _u64, _u64, _u32, _i32, _vp, _u32, _vp, _u32, _i32, C.c_double, _vp],
     "brc_timing_enable": [_vp, _i32],

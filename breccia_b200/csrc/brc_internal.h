@@ -203,6 +203,7 @@ struct brc_kv8_attn_args {
     uint32_t table_stride = 0;
     const uint32_t *seq_lens = nullptr;
     const uint32_t *cu_q = nullptr;
+    uint32_t total_q = UINT32_MAX;   // rows of q and out, where a caller says (with cu_q)
     uint32_t n_seqs = 0, max_seq_len = 0, max_q = 1;
     float scale = 0.f;
     void *out = nullptr;

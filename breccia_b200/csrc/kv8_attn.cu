@@ -56,6 +56,7 @@ struct AttnParams {
     uint64_t page_bytes;
     uint32_t q_dtype, out_dtype, gate_head_stride;
     uint32_t table_stride, n_seqs, max_seq_len, max_q, n_pages, page0;   // page0: layer * n_pages
+    uint32_t total_q;        // rows of q and out behind which cu_q must not lead
     uint32_t n_head, n_kv, group, kvb, row_groups;                        // row_groups: warps that split a pass's rows
     uint32_t pass_rows, passes, units_per_seq, n_stages, q_bufs, unit_cost;
     float scale_log2;
@@ -91,10 +92,19 @@ __host__ __device__ inline Smem smem_layout(uint32_t hd, uint32_t warps, uint32_
     return s;
 }
 
-__device__ __forceinline__ uint32_t tokens_of(const AttnParams &p, uint32_t s) { return p.cu_q ? p.cu_q[s + 1] - p.cu_q[s] : p.max_q; }
+// T of a sequence (none where its prefix goes backwards), and how many of its tokens the call has rows for.
+__device__ __forceinline__ uint32_t tokens_of(const AttnParams &p, uint32_t s) {
+    if (!p.cu_q) return p.max_q;
+    const uint32_t b = p.cu_q[s], e = p.cu_q[s + 1];
+    return e > b ? e - b : 0u;
+}
+__device__ __forceinline__ uint32_t rows_of(const AttnParams &p, uint32_t s) {
+    const uint32_t t = min(tokens_of(p, s), p.max_q);
+    return p.cu_q ? min(t, p.total_q - min(p.cu_q[s], p.total_q)) : t;
+}
 __device__ __forceinline__ uint32_t cells_of(const AttnParams &p, uint32_t s) { return min(p.seq_lens[s], p.max_seq_len); }
 __device__ __forceinline__ uint32_t pages_of(const AttnParams &p, uint32_t s) {
-    return tokens_of(p, s) ? (cells_of(p, s) + 15u) / 16u : 0u;
+    return rows_of(p, s) ? (cells_of(p, s) + 15u) / 16u : 0u;
 }
 // What a unit counts for when the work is cut: its pages and, in front of them, what starting and finishing a unit costs.
 // (The host refuses a call whose costs could add up to 2^31.)
@@ -193,7 +203,7 @@ __device__ __forceinline__ void stage_q(const AttnParams &p, const Smem &L, uint
     const uint32_t hg = g.u / p.passes, pass = g.u % p.passes;
     const uint32_t n_q = tokens_of(p, g.s), len = cells_of(p, g.s);
     const uint64_t tok0 = p.cu_q ? p.cu_q[g.s] : (uint64_t)g.s * p.max_q;
-    const uint32_t rows = min(n_q, p.max_q) * p.group, all = p.kvb * p.pass_rows, d = lane % LANES * 8u;
+    const uint32_t rows = rows_of(p, g.s) * p.group, all = p.kvb * p.pass_rows, d = lane % LANES * 8u;
     float *row_fac = reinterpret_cast<float *>(smem + L.row_fac) + buf * all;
     uint32_t *row_vis = reinterpret_cast<uint32_t *>(smem + L.row_vis) + buf * p.pass_rows;
     for (uint32_t r0 = w * SET + lane / LANES; r0 / SET * SET < all; r0 += n_w * SET * U) {   // (all is a multiple of SET: whole warps)
@@ -285,6 +295,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
             if (blockIdx.x == 0) {
                 if (p.seq_lens[s] > p.max_seq_len) { atomicOr(p.status, BRC_DEV_BAD_POS); p.status[1] = p.seq_lens[s]; }
                 if (tokens_of(p, s) > p.max_q) { atomicOr(p.status, BRC_DEV_BAD_POS); p.status[1] = tokens_of(p, s); }
+                if (p.cu_q && (p.cu_q[s + 1] > p.total_q || p.cu_q[s + 1] < p.cu_q[s])) { atomicOr(p.status, BRC_DEV_BAD_POS); p.status[1] = p.cu_q[s + 1]; }
             }
         }
         run = sum;
@@ -433,7 +444,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
         const uint32_t hg = g.u / p.passes, pass = g.u % p.passes;
         const uint32_t n_q = tokens_of(p, g.s), len = cells_of(p, g.s);
         const uint64_t tok0 = p.cu_q ? p.cu_q[g.s] : (uint64_t)g.s * p.max_q;
-        const uint32_t rows = min(n_q, p.max_q) * p.group;               // of a kv head, over all passes
+        const uint32_t rows = rows_of(p, g.s) * p.group;                 // of a kv head, over all passes
         const uint32_t vis_min = len + 1u > n_q ? len + 1u - n_q : 0u;   // cells that every row sees
         const uint32_t buf_q = idx % p.q_bufs;
         float ks_now = 1.f, ev_now = 0.f, ks_next = 1.f, ev_next = 0.f;
@@ -764,7 +775,7 @@ __global__ void __launch_bounds__(W * ROWS * 32) kv8_merge_kernel(const AttnPara
     const uint32_t warp = W == 1 ? 0u : threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const uint32_t hg = u / p.passes, pass = u % p.passes, row = blockIdx.y * ROWS + (W == 1 ? threadIdx.x >> 5 : 0u);
     const uint32_t h = row / p.pass_rows, r = row % p.pass_rows, gr_row = pass * p.pass_rows + r;
-    if (row >= p.kvb * p.pass_rows || gr_row >= min(tokens_of(p, s), p.max_q) * p.group) return;   // whole warps; W > 1: the whole CTA
+    if (row >= p.kvb * p.pass_rows || gr_row >= rows_of(p, s) * p.group) return;   // whole warps; W > 1: the whole CTA
     const uint32_t n = all ? c1 - c0 + 1u : 0u;
 
     float m = NONE, wm = NONE, l = 0.f, v[PER];
@@ -1008,6 +1019,7 @@ brc_status brc_kv8_attend(brc_pool *pool, const char *who, const brc_kv8_attn_ar
     p.n_seqs = a.n_seqs;
     p.max_seq_len = a.max_seq_len;
     p.max_q = a.max_q;
+    p.total_q = a.total_q;
     p.n_pages = pool->n_pages;
     p.page0 = a.layer * pool->n_pages;
     p.n_head = a.n_head;
@@ -1053,30 +1065,26 @@ brc_status brc_kv8_attn_workspace_bytes(const brc_pool *pool, uint32_t n_seqs, u
     return brc_kv8_workspace(pool, n_seqs, n_head, max_q, out_bytes);
 }
 
-brc_status brc_kv8_attn(brc_pool *pool, uint32_t layer, const void *q_dev, int32_t q_dtype, uint32_t n_head, const float *gate_dev,
-                        uint32_t gate_head_stride, const uint32_t *block_tables_dev, uint32_t table_stride,
+brc_status brc_kv8_attn(brc_pool *pool, uint32_t layer, const void *q_dev, int32_t q_dtype, uint32_t n_head,
+                        const float *gate_dev, uint32_t gate_head_stride, const uint32_t *block_tables_dev, uint32_t table_stride,
                         const uint32_t *seq_lens_dev, const uint32_t *cu_q_dev, uint32_t n_seqs, uint32_t max_q, uint32_t max_seq_len,
                         float scale, void *out_dev, int32_t out_dtype, void *workspace_dev, uint64_t workspace_bytes, void *stream) {
-    brc_kv8_attn_args a;
-    a.layer = layer;
-    a.q = q_dev;
-    a.q_dtype = q_dtype;
-    a.n_head = n_head;
-    a.gate = gate_dev;
-    a.gate_head_stride = gate_head_stride;
-    a.block_tables = block_tables_dev;
-    a.table_stride = table_stride;
-    a.seq_lens = seq_lens_dev;
-    a.cu_q = cu_q_dev;
-    a.n_seqs = n_seqs;
-    a.max_q = max_q;
-    a.max_seq_len = max_seq_len;
-    a.scale = scale;
-    a.out = out_dev;
-    a.out_dtype = out_dtype;
-    a.workspace = workspace_dev;
-    a.workspace_bytes = workspace_bytes;
+    brc_kv8_attn_args a = {layer,    q_dev,    q_dtype, n_head,      gate_dev, gate_head_stride, block_tables_dev, table_stride,  seq_lens_dev,
+                           cu_q_dev, UINT32_MAX, n_seqs, max_seq_len, max_q,    scale,            out_dev,          out_dtype,     workspace_dev,
+                           workspace_bytes};
     return brc_kv8_attend(pool, "brc_kv8_attn", a, stream);
+}
+
+brc_status brc_kv8_attn_ragged(brc_pool *pool, uint32_t layer, const void *q_dev, int32_t q_dtype, uint32_t total_q, uint32_t n_head,
+                               const float *gate_dev, uint32_t gate_head_stride, const uint32_t *block_tables_dev,
+                               uint32_t table_stride, const uint32_t *seq_lens_dev, const uint32_t *cu_q_dev, uint32_t n_seqs,
+                               uint32_t max_q, uint32_t max_seq_len, float scale, void *out_dev, int32_t out_dtype, void *workspace_dev,
+                               uint64_t workspace_bytes, void *stream) {
+    if (!cu_q_dev) return brc_fail(BRC_ERR_INVALID, "brc_kv8_attn_ragged: NULL prefix of the sequences' rows");
+    brc_kv8_attn_args a = {layer,    q_dev,   q_dtype, n_head,      gate_dev, gate_head_stride, block_tables_dev, table_stride,  seq_lens_dev,
+                           cu_q_dev, total_q, n_seqs,  max_seq_len, max_q,    scale,            out_dev,          out_dtype,     workspace_dev,
+                           workspace_bytes};
+    return brc_kv8_attend(pool, "brc_kv8_attn_ragged", a, stream);
 }
 
 }  // extern "C"

@@ -644,7 +644,7 @@ def kv8_attend(pool: KvPool, layer: int, q: torch.Tensor, block_tables: torch.Te
                out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None, gate: torch.Tensor | None = None,
                gate_head_stride: int = 0, stream=None) -> torch.Tensor:
     """Attention over an 8-bit pool for the last T tokens of each sequence (brc_kv8_attn): q [tokens, n_head, hd], T = max_q, or
-    ragged by cu_q [n_seqs + 1] int32 with T <= max_q; token i of T sees seq_lens[s] - (T - 1 - i) cells.  Sums and softmax
+    ragged by cu_q [n_seqs + 1] int32 with T <= max_q (rows past q's end are left out and reported by check()); token i of T sees seq_lens[s] - (T - 1 - i) cells.  Sums and softmax
     in f32, probabilities to 22 bits, one rounding to `out_dtype` (q's type unless given).  `out` may be q.
     `workspace` from kv8_workspace; calls that may run at the same time need one each."""
     device = pool.device
@@ -672,8 +672,9 @@ def kv8_attend(pool: KvPool, layer: int, q: torch.Tensor, block_tables: torch.Te
     if workspace.get_device() != device or (gate is not None and (gate.get_device() != device or gate.dtype != torch.float32)):
         raise BrcError(_lib.ERR_INVALID, f"kv8_attend: workspace on {workspace.device}, gate {None if gate is None else (gate.dtype, gate.device)}: "
                                          f"cuda:{device} and float32 wanted")
-    _lib.check(_lib.load().brc_kv8_attn(
-        pool.handle, layer, q.data_ptr(), _dtype(q.dtype, "kv8_attend"), n_head, None if gate is None else gate.data_ptr(), gate_head_stride,
+    L, rows = _lib.load(), () if cu is None else (tokens,)
+    _lib.check((L.brc_kv8_attn if cu is None else L.brc_kv8_attn_ragged)(
+        pool.handle, layer, q.data_ptr(), _dtype(q.dtype, "kv8_attend"), *rows, n_head, None if gate is None else gate.data_ptr(), gate_head_stride,
         _words(block_tables, device, "kv8_attend: block_tables"), stride, _words(seq_lens, device, "kv8_attend: seq_lens", n_seqs), cu, n_seqs, max_q,
         max_seq_len, 1.0 / math.sqrt(hd) if scale is None else scale, out.data_ptr(), _dtype(out.dtype, "kv8_attend"), workspace.data_ptr(),
         workspace.nbytes, _raw_stream(stream, device)))

@@ -124,7 +124,7 @@ BRC_API brc_status brc_pool_v_layout(const brc_pool *pool, int32_t *out_layout);
  * and side, always a power of two 2^e with -120 <= e <= 120.  Codes are e4m3
  * (finite ones only: |code| <= 448) or signed bytes (|code| <= 127).  1040 bytes
  * of K and V per cell instead of 2048 at 2 kv heads of 256.  Built for such a pool:
- * brc_kv8_append / brc_kv8_read / brc_kv8_attn below; brc_kv_append (f32 or f16
+ * brc_kv8_append / brc_kv8_read / brc_kv8_attn(_ragged) below; brc_kv_append (f32 or f16
  * sources) and brc_paged_decode_attn, which call them; brc_page_copy,
  * brc_seq_fork, brc_tier_*, brc_cold_* and brc_pool_read / _write / _zero (whole
  * pages, scales included); the allocator and the prefix tree.  Every other entry
@@ -395,6 +395,16 @@ BRC_API brc_status brc_kv8_attn(brc_pool *pool, uint32_t layer, const void *q_de
                                 uint32_t table_stride, const uint32_t *seq_lens_dev, const uint32_t *cu_q_dev,
                                 uint32_t n_seqs, uint32_t max_q, uint32_t max_seq_len, float scale, void *out_dev,
                                 int32_t out_dtype, void *workspace_dev, uint64_t workspace_bytes, void *stream);
+/* brc_kv8_attn with a prefix, told how many rows q and out have: what cu_q_dev
+ * says of rows at or past total_q is left out, neither read nor written, and
+ * reported through brc_pool_check, as is a prefix that goes backwards (no rows for that
+ * sequence).  brc_kv8_attn itself takes cu_q_dev at its word. */
+BRC_API brc_status brc_kv8_attn_ragged(brc_pool *pool, uint32_t layer, const void *q_dev, int32_t q_dtype, uint32_t total_q,
+                                       uint32_t n_head, const float *gate_dev, uint32_t gate_head_stride,
+                                       const uint32_t *block_tables_dev, uint32_t table_stride,
+                                       const uint32_t *seq_lens_dev, const uint32_t *cu_q_dev, uint32_t n_seqs,
+                                       uint32_t max_q, uint32_t max_seq_len, float scale, void *out_dev,
+                                       int32_t out_dtype, void *workspace_dev, uint64_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------- rotary positions
  * The rotation of Qsa::rope_q / rope_k (crates/breccia-kernels/src/qsa/mod.rs:

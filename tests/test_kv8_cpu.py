@@ -129,3 +129,17 @@ def test_pool_refusals():
     for null in (lambda: L.brc_kv8_append(None, 0, d, 4, d, 1, 1, None, 1, 1, d, 0, d, 0, 0, None, 0, 0, 1.0, None),
                  lambda: L.brc_kv8_attn_workspace_bytes(None, 1, 16, 1, C.byref(b)), lambda: L.brc_pool_kv8_code(None, C.byref(code))):
         assert null() == _lib.ERR_INVALID
+
+
+def test_ragged_attention_refusals():
+    L = _lib.load()
+    from breccia_b200.qsa import KvPool
+
+    book, d = KvPool(0, 1, 2, 256, 8, bookkeeping_only=True), C.c_void_p(0x1000)
+
+    def call(pool=book.handle, total=3, cu=d):
+        return L.brc_kv8_attn_ragged(pool, 0, d, 1, total, 16, None, 0, d, 4, d, cu, 1, 3, 16, 1.0, d, 1, d, 1 << 30, None)
+
+    assert call() == _lib.ERR_CUDA and b"brc_kv8_attn_ragged" in L.brc_last_error()
+    assert call(cu=None) == _lib.ERR_INVALID and b"NULL prefix" in L.brc_last_error()
+    assert call(pool=None) == _lib.ERR_INVALID

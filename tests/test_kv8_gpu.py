@@ -758,3 +758,32 @@ def test_sixteen_bit_results_are_rounded_once(cuda_device, code, dt, n_head, n_k
             err = np.abs(got[s * max_q + i] - want)
             assert (err <= tol).all(), (s, i, float((err - tol).max()), float(err.max()))
     pool.release()
+
+
+@pytest.mark.parametrize("n_head,max_q", [(8, 4), (40, 4)])   # 16 rows; 80: three passes
+def test_a_prefix_that_leads_past_the_rows(cuda_device, n_head, max_q):
+    """cu_q of another step: rows that q and out do not have are neither read nor written, a prefix that goes backwards is no rows; both
+    reported, and what is there is as it would be."""
+    lens = [700, 90, 33]
+    tables, n_pages = scattered(5, lens)
+    pool = KvPool(0, 1, 2, 128, n_pages, kv8="int8")
+    fill(pool, 3)
+    ws, big = kv8_workspace(pool, 3, n_head, max_q), torch.randn(12, n_head, 128, device="cuda")
+
+    def call(rows, cu):
+        q, out = big.clone(), torch.full_like(big, 7.0)
+        q[rows:] = NAN
+        kv8_attend(pool, 0, q[:rows], dev(tables), dev(lens), 700, ws, max_q=max_q, cu_q=dev(cu), out=out[:rows])
+        return out
+
+    want = call(10, [0, 4, 6, 10])
+    pool.check()
+    assert (want[10:] == 7).all() and torch.isfinite(want[:10]).all()
+    for rows, cu, live in ((8, [0, 4, 6, 10], 8), (5, [0, 4, 6, 10], 5), (10, [0, 4, 6, 2 ** 31 - 1], 6), (8, [0, 4, 9, 12], 4), (6, [0, 4, 2, 2], 4)):
+        got = call(rows, cu)
+        with pytest.raises(BrcError, match="position past bound"):
+            pool.check()
+        # f32 sums in another order where the cut moved: far apart only if a row saw other cells
+        assert torch.allclose(got[:live], want[:live], rtol=1e-4, atol=1e-4) and (got[rows:] == 7).all()
+    pool.check()
+    pool.release()
