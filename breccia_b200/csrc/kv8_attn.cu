@@ -984,7 +984,7 @@ brc_status brc_kv8_attend(brc_pool *pool, const char *who, const brc_kv8_attn_ar
                         a.max_seq_len, (unsigned long long)capacity, a.table_stride, pool->page_tokens);
     if (a.gate && a.gate_head_stride < pool->head_dim)
         return brc_fail(BRC_ERR_INVALID, "%s: gate_head_stride %u < head_dim %u", who, a.gate_head_stride, pool->head_dim);
-    if (a.n_seqs == 0 || a.max_q == 0) return BRC_OK;
+    if (a.n_seqs == 0 || a.max_q == 0 || a.total_q == 0) return BRC_OK;
     if (!a.q || !a.block_tables || !a.seq_lens || !a.out)
         return brc_fail(BRC_ERR_INVALID, "%s: NULL query, block table, length or output pointer", who);
     if ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.workspace)) & 15u)

@@ -787,3 +787,14 @@ def test_a_prefix_that_leads_past_the_rows(cuda_device, n_head, max_q):
         assert torch.allclose(got[:live], want[:live], rtol=1e-4, atol=1e-4) and (got[rows:] == 7).all()
     pool.check()
     pool.release()
+
+
+def test_a_ragged_batch_without_tokens(cuda_device):
+    """No sequence has a token this step: an empty q (whose address is 0) is an empty result, as in the append."""
+    pool = KvPool(0, 1, 2, 128, 4, kv8="int8")
+    t, lens, cu, q = dev([[0], [1], [2]]), dev([3, 16, 0]), dev([0, 0, 0, 0]), torch.ones(0, 8, 128, device="cuda")
+    assert kv8_attend(pool, 0, q, t, lens, 16, kv8_workspace(pool, 3, 8, 4), max_q=4, cu_q=cu).shape == (0, 8, 128)
+    with pytest.raises(BrcError):
+        kv8_attend(pool, 1, q, t, lens, 16, kv8_workspace(pool, 3, 8, 4), max_q=4, cu_q=cu)   # checked all the same
+    pool.check()
+    pool.release()
