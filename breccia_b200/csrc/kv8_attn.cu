@@ -58,7 +58,7 @@ struct AttnParams {
     uint32_t table_stride, n_seqs, max_seq_len, max_q, n_pages, page0;   // page0: layer * n_pages
     uint32_t total_q;        // rows of q and out behind which cu_q must not lead
     uint32_t n_head, n_kv, group, kvb, row_groups;                        // row_groups: warps that split a pass's rows
-    uint32_t pass_rows, passes, units_per_seq, n_stages, q_bufs, unit_cost;
+    uint32_t pass_rows, head_groups, units_per_seq, n_stages, q_bufs, unit_cost;   // units_per_seq: the longest q's
     float scale_log2;
 };
 
@@ -106,9 +106,21 @@ __device__ __forceinline__ uint32_t cells_of(const AttnParams &p, uint32_t s) { 
 __device__ __forceinline__ uint32_t pages_of(const AttnParams &p, uint32_t s) {
     return rows_of(p, s) ? (cells_of(p, s) + 15u) / 16u : 0u;
 }
+// Passes that a sequence's own rows fill (at least one), and its units: kv-head groups x passes.  MANY: the call's longest sequence fills
+// more than one; known at compile time, since the divisions by it would add 0.3 to 1 us in front of the first page of every other call.
+template <bool MANY>
+__device__ __forceinline__ uint32_t passes_of(const AttnParams &p, uint32_t s) {
+    return MANY ? max((rows_of(p, s) * p.group + PASS_ROWS - 1u) / PASS_ROWS, 1u) : 1u;
+}
+template <bool MANY>
+__device__ __forceinline__ uint32_t units_of(const AttnParams &p, uint32_t s) { return p.head_groups * passes_of<MANY>(p, s); }
 // What a unit counts for when the work is cut: its pages and, in front of them, what starting and finishing a unit costs.
 // (The host refuses a call whose costs could add up to 2^31.)
-__device__ __forceinline__ uint32_t cost_of(const AttnParams &p, uint32_t pages) { return pages ? (pages + p.unit_cost) * p.units_per_seq : 0u; }
+template <bool MANY>
+__device__ __forceinline__ uint32_t cost_of(const AttnParams &p, uint32_t s) {
+    const uint32_t pages = pages_of(p, s);
+    return pages ? (pages + p.unit_cost) * units_of<MANY>(p, s) : 0u;
+}
 __device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t grid) { return max((total + grid - 1u) / grid, MIN_SHARE); }
 
 __device__ __forceinline__ void store_out(const AttnParams &p, uint64_t at, float a, float b, float c, float d) {
@@ -158,11 +170,11 @@ __device__ __forceinline__ void load_q8(const AttnParams &p, uint64_t at, float 
 
 // A share's walk over the units: [lo, hi) on the axis of costs, and where the unit in hand begins on it.
 struct Cursor {
-    uint32_t at, lo, hi, s, u;
+    uint32_t at, lo, hi, s, hg, pass;
 };
 
-struct Segment {
-    uint32_t s, u, pg, n, pages;
+struct Segment {   // pages [pg, pg + n) of one unit: kv-head group hg of sequence s, pass `pass` of its rows
+    uint32_t s, hg, pass, pg, n, pages;
 };
 
 struct Start {   // of a share: its first segment (n = 0: none) and where to go on
@@ -170,23 +182,28 @@ struct Start {   // of a share: its first segment (n = 0: none) and where to go 
     Segment seg;
 };
 
+template <bool MANY>
 __device__ __forceinline__ bool next_segment(const AttnParams &p, Cursor &c, Segment &g) {
     while (c.at < c.hi) {
         const uint32_t pages = pages_of(p, c.s);
-        if (pages == 0 || c.u == p.units_per_seq) {
+        if (pages == 0 || c.hg == p.head_groups) {
             ++c.s;
-            c.u = 0;
+            c.hg = 0;
             continue;
         }
         const uint32_t first = c.at + p.unit_cost;   // page 0's place on the axis
         const uint32_t from = min(c.lo > first ? c.lo - first : 0u, pages), to = min(c.hi > first ? c.hi - first : 0u, pages);
         g.s = c.s;
-        g.u = c.u;
+        g.hg = c.hg;
+        g.pass = MANY ? c.pass : 0u;
         g.pages = pages;
         g.pg = from;
         g.n = to > from ? to - from : 0u;
         c.at = first + pages;
-        ++c.u;
+        if (!MANY || ++c.pass == passes_of<MANY>(p, g.s)) {
+            c.pass = 0;
+            ++c.hg;
+        }
         if (g.n) return true;   // a share may end inside a unit's cost, in front of its first page
     }
     return false;
@@ -200,7 +217,7 @@ template <int HD, bool SPLIT_Q, int U, class F>
 __device__ __forceinline__ void stage_q(const AttnParams &p, const Smem &L, uint8_t *smem, const Segment &g, uint32_t buf, uint32_t w,
                                         uint32_t n_w, uint32_t lane, F &&meanwhile) {
     constexpr uint32_t LANES = HD / 8, SET = 32 / LANES;
-    const uint32_t hg = g.u / p.passes, pass = g.u % p.passes;
+    const uint32_t hg = g.hg, pass = g.pass;
     const uint32_t n_q = tokens_of(p, g.s), len = cells_of(p, g.s);
     const uint64_t tok0 = p.cu_q ? p.cu_q[g.s] : (uint64_t)g.s * p.max_q;
     const uint32_t rows = rows_of(p, g.s) * p.group, all = p.kvb * p.pass_rows, d = lane % LANES * 8u;
@@ -260,6 +277,7 @@ template <int HD, uint32_t CODE, bool SPLIT_Q, int RT, int RG, int KVB, int W>
 __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_constant__ CUtensorMap tm, const AttnParams p) {
     constexpr uint32_t SLABS = HD / 128, CONSUMERS = W * 32, ROW = HD + 4;
     constexpr uint32_t STEP = KVB * RG, LANES = W / STEP, PASS = RG * RT * 8, STAGE = KVB * 2 * 16 * HD, SLAB = STAGE / SLABS;   // LANES: warps that take pages in turn
+    constexpr bool MANY = RG == 2;   // more than PASS_ROWS rows take the widest form
     static_assert(W % STEP == 0 && CONSUMERS % (HD / 4) == 0, "");
     extern __shared__ __align__(1024) uint8_t smem[];
     const Smem L = smem_layout(HD, W, KVB, PASS, SPLIT_Q, p.n_stages, p.q_bufs);
@@ -291,7 +309,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
         for (uint32_t i = 0; i < per_thread; ++i) {
             const uint32_t s = tid * per_thread + i;
             if (s >= p.n_seqs) break;
-            sum += cost_of(p, pages_of(p, s));
+            sum += cost_of<MANY>(p, s);
             if (blockIdx.x == 0) {
                 if (p.seq_lens[s] > p.max_seq_len) { atomicOr(p.status, BRC_DEV_BAD_POS); p.status[1] = p.seq_lens[s]; }
                 if (tokens_of(p, s) > p.max_q) { atomicOr(p.status, BRC_DEV_BAD_POS); p.status[1] = tokens_of(p, s); }
@@ -319,15 +337,15 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
         if (lo < hi && at <= lo && lo < at + sum) {
             uint32_t a = at, c;
             uint32_t s = tid * per_thread;
-            while (a + (c = cost_of(p, pages_of(p, s))) <= lo) {
+            while (a + (c = cost_of<MANY>(p, s)) <= lo) {
                 a += c;
                 ++s;
             }
-            c /= p.units_per_seq;
-            const uint32_t u = (lo - a) / c;
-            Cursor first{a + u * c, lo, hi, s, u};
+            c /= units_of<MANY>(p, s);
+            const uint32_t u = (lo - a) / c, passes = passes_of<MANY>(p, s), hg = u / passes;
+            Cursor first{a + u * c, lo, hi, s, hg, u - hg * passes};
             Segment seg = {};
-            seg.n = next_segment(p, first, seg) ? seg.n : 0u;
+            seg.n = next_segment<MANY>(p, first, seg) ? seg.n : 0u;
             start->cur = first;
             start->seg = seg;
         }
@@ -336,7 +354,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
             for (uint32_t i = 0; i < per_thread; ++i) {
                 const uint32_t s = tid * per_thread + i;
                 if (s >= p.n_seqs) break;
-                at += cost_of(p, pages_of(p, s));
+                at += cost_of<MANY>(p, s);
                 p.prefix[s + 1] = at;
             }
         }
@@ -356,7 +374,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
         if (warp > W) {
             // -------------------------------------------------------------- helpers: q of every unit but the first
             uint32_t idx = 0;
-            for (; more; more = next_segment(p, cur, g)) {
+            for (; more; more = next_segment<MANY>(p, cur, g)) {
                 if (idx) {
                     const uint32_t buf = idx % p.q_bufs;
                     if (idx >= p.q_bufs) ok = brc::mbar_wait(q_empty0 + 8u * buf, (idx - p.q_bufs) / p.q_bufs & 1u);
@@ -374,8 +392,8 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
             const uint64_t policy = brc::l2_policy_evict_first();
             const uint32_t j = lane / SLABS, sl = lane % SLABS;
             uint32_t stage = 0, parity = 1;   // the first round finds every stage empty
-            for (; ok && more; more = next_segment(p, cur, g)) {
-                const uint32_t row0 = (g.u / p.passes) * KVB * 16u;
+            for (; ok && more; more = next_segment<MANY>(p, cur, g)) {
+                const uint32_t row0 = g.hg * KVB * 16u;
                 const uint32_t *table = p.block_tables + (uint64_t)g.s * p.table_stride + g.pg;
                 uint32_t ahead = lane < g.n ? table[lane] : 0u;
                 for (uint32_t i0 = 0; ok && i0 < g.n; i0 += 32u) {
@@ -424,7 +442,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
     };
     auto scales_of = [&](const Segment &g, uint32_t id, float &ks, float &ev) {
         if (id < p.n_pages) {
-            const uint64_t at = id * p.page_bytes + code_bytes + (g.u / p.passes * KVB + hk) * 4u;
+            const uint64_t at = id * p.page_bytes + code_bytes + (g.hg * KVB + hk) * 4u;
             ks = *reinterpret_cast<const float *>(p.k_layer + at);
             ev = (float)brc::kv8_scale_exponent(*reinterpret_cast<const float *>(p.v_layer + at));
         } else {
@@ -441,7 +459,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
     Segment g_next;
     uint32_t ids = more ? ids_of(g, pl) : 0u;
     while (more) {
-        const uint32_t hg = g.u / p.passes, pass = g.u % p.passes;
+        const uint32_t hg = g.hg, pass = g.pass;
         const uint32_t n_q = tokens_of(p, g.s), len = cells_of(p, g.s);
         const uint64_t tok0 = p.cu_q ? p.cu_q[g.s] : (uint64_t)g.s * p.max_q;
         const uint32_t rows = rows_of(p, g.s) * p.group;                 // of a kv head, over all passes
@@ -673,7 +691,7 @@ __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_
             }
         const bool whole = g.n == g.pages;
         const uint64_t slot = (2ull * blockIdx.x + (g.pg == 0 ? 1u : 0u)) * (KVB * PASS);
-        more = next_segment(p, cur, g_next);
+        more = next_segment<MANY>(p, cur, g_next);
         if (more) ids = ids_of(g_next, (pl + LANES - done % LANES) % LANES);   // on their way while this unit is merged
         brc::named_bar_sync(1, CONSUMERS);
 #pragma unroll
@@ -759,7 +777,7 @@ __device__ __forceinline__ void load_if(bool live, const float *at, float4 &v) {
 // The partials that the shares' boundaries left of each (unit, query row), merged in share order; zeros for a sequence without
 // cells.  Units that one share covered are finished already.  W warps per row, ROWS rows per CTA, B partials of a warp
 // in flight (their sums and exponents together: one round trip).
-template <int HD, int W, int ROWS, int B>
+template <int HD, int W, int ROWS, int B, bool MANY>
 __global__ void __launch_bounds__(W * ROWS * 32) kv8_merge_kernel(const AttnParams p, uint32_t grid) {
     constexpr uint32_t PER = HD / 32;
     __shared__ float part[W == 1 ? 1 : W][HD];
@@ -768,12 +786,14 @@ __global__ void __launch_bounds__(W * ROWS * 32) kv8_merge_kernel(const AttnPara
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t s = blockIdx.x / p.units_per_seq, u = blockIdx.x % p.units_per_seq;
     const uint32_t before = p.prefix[s], all = p.prefix[s + 1] - before;
-    const uint32_t share = share_of(p.prefix[p.n_seqs], grid), unit = all / p.units_per_seq;
+    const uint32_t units = units_of<MANY>(p, s);
+    if (u >= units) return;   // the longest sequence's passes, not this one's
+    const uint32_t share = share_of(p.prefix[p.n_seqs], grid), unit = all / units;
     const uint32_t begin = before + u * unit + p.unit_cost;   // page 0
     const uint32_t c0 = begin / share, c1 = all ? (begin + unit - p.unit_cost - 1u) / share : c0;
     if (all && c0 == c1) return;
     const uint32_t warp = W == 1 ? 0u : threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const uint32_t hg = u / p.passes, pass = u % p.passes, row = blockIdx.y * ROWS + (W == 1 ? threadIdx.x >> 5 : 0u);
+    const uint32_t passes = passes_of<MANY>(p, s), hg = u / passes, pass = u % passes, row = blockIdx.y * ROWS + (W == 1 ? threadIdx.x >> 5 : 0u);
     const uint32_t h = row / p.pass_rows, r = row % p.pass_rows, gr_row = pass * p.pass_rows + r;
     if (row >= p.kvb * p.pass_rows || gr_row >= rows_of(p, s) * p.group) return;   // whole warps; W > 1: the whole CTA
     const uint32_t n = all ? c1 - c0 + 1u : 0u;
@@ -931,11 +951,11 @@ brc_status launch(const brc_pool *pool, AttnParams p, uint32_t grid, uint32_t me
         // Few units have many partials each (one long sequence: one from every SM): 16 warps a row fetch eighty at a time.
         cfg.gridDim = dim3(p.n_seqs * p.units_per_seq, merge_rows);
         cfg.blockDim = dim3(512);
-        BRC_CUDA(cudaLaunchKernelEx(&cfg, kv8_merge_kernel<HD, 16, 1, 5>, p, grid));
+        BRC_CUDA(cudaLaunchKernelEx(&cfg, kv8_merge_kernel<HD, 16, 1, 5, RG == 2>, p, grid));
     } else {   // many units have a few: a warp a row
         cfg.gridDim = dim3(p.n_seqs * p.units_per_seq, (merge_rows + 7u) / 8u);
         cfg.blockDim = dim3(256);
-        BRC_CUDA(cudaLaunchKernelEx(&cfg, kv8_merge_kernel<HD, 1, 8, 6>, p, grid));
+        BRC_CUDA(cudaLaunchKernelEx(&cfg, kv8_merge_kernel<HD, 1, 8, 6, RG == 2>, p, grid));
     }
     return BRC_OK;
 }
@@ -1028,7 +1048,7 @@ brc_status brc_kv8_attend(brc_pool *pool, const char *who, const brc_kv8_attn_ar
     p.kvb = s.kvb;
     p.row_groups = s.row_groups;
     p.pass_rows = s.pass_rows;
-    p.passes = s.passes;
+    p.head_groups = pool->n_kv_head / s.kvb;
     p.units_per_seq = s.units_per_seq;
     p.scale_log2 = a.scale * 1.4426950408889634f;
     // Starting and finishing a unit takes a CTA about as long as streaming 128 KiB for each of the unit's heads, half as much again where

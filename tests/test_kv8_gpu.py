@@ -798,3 +798,43 @@ def test_a_ragged_batch_without_tokens(cuda_device):
         kv8_attend(pool, 1, q, t, lens, 16, kv8_workspace(pool, 3, 8, 4), max_q=4, cu_q=cu)   # checked all the same
     pool.check()
     pool.release()
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+@pytest.mark.parametrize("n_head,n_kv,hd,n_q", [(40, 2, 128, [1, 1, 8, 0, 1, 3, 1, 8]), (16, 2, 256, [1, 9, 1, 0, 4, 1, 5, 1]), (5, 1, 256, [0, 1, 0, 16, 7, 1, 2, 1])])
+def test_sequences_take_the_passes_of_their_own_rows(cuda_device, code, dt, n_head, n_kv, hd, n_q):
+    tables, n_pages = scattered(2, LENS)
+    pool = KvPool(0, 1, n_kv, hd, n_pages, kv8=code)
+    values = fill(pool, 4)
+    run_and_compare(pool, values, tables, LENS, n_q, n_head, dt, dt, True, gate=True)
+    pool.release()
+
+
+def test_short_drafts_beside_a_long_one_stream_their_cache_once(cuda_device):
+    """One sequence of 8 tokens (160 rows, five passes) beside 31 of one (20 rows, one pass): close to a call of 32 sequences of one token
+    (36 streams against 32), and far from five passes for everybody (160 against 32)."""
+    n, cells_each, n_head = 32, 16384, 40
+    pool = KvPool(0, 1, 2, 128, n * cells_each // 16, kv8="int8")
+    tables, lens = dev(np.arange(n * cells_each // 16).reshape(n, -1)), dev([cells_each] * n)
+    n_q = [1] * (n - 1) + [8]
+    q, ws = torch.randn(sum(n_q), n_head, 128, device="cuda").half(), kv8_workspace(pool, n, n_head, 8)
+
+    def ms(call):
+        times = []
+        for _ in range(9):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda._sleep(200_000)      # the call is issued while the GPU is still busy
+            a.record()
+            call()
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return sorted(times)[4]
+
+    cu = dev(np.concatenate([[0], np.cumsum(n_q)]))
+    one = ms(lambda: kv8_attend(pool, 0, q[:n], tables, lens, cells_each, ws))
+    mixed = ms(lambda: kv8_attend(pool, 0, q, tables, lens, cells_each, ws, max_q=8, cu_q=cu))
+    assert mixed < 2.2 * one, (one, mixed)   # geometric middle of 36 / 32 and 160 / 32: 2.4
+    pool.check()
+    pool.release()
