@@ -133,12 +133,19 @@ __device__ __forceinline__ void store_out(const AttnParams &p, uint64_t at, floa
     }
 }
 
+// As in the binary16 decode attention.  (With __expf the result would be off by 2^-18 of itself at -80, and zero below -89.)
+__device__ __forceinline__ float sigmoid_f32(float x) {
+    if (x >= 0.f) return 1.f / (1.f + expf(-x));
+    const float e = expf(x);
+    return e / (1.f + e);
+}
+
 // Four values of one output row, gated and stored.  `head_row`: token * n_head + head.
 __device__ __forceinline__ void finish_row(const AttnParams &p, uint32_t hd, uint64_t head_row, uint32_t d, float (&v)[4]) {
     if (p.gate) {
         const float *g = p.gate + head_row * p.gate_head_stride + d;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] *= 1.f / (1.f + __expf(-g[i]));
+        for (int i = 0; i < 4; ++i) v[i] *= sigmoid_f32(g[i]);
     }
     store_out(p, head_row * hd + d, v[0], v[1], v[2], v[3]);
 }

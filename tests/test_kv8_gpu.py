@@ -838,3 +838,21 @@ def test_short_drafts_beside_a_long_one_stream_their_cache_once(cuda_device):
     assert mixed < 2.2 * one, (one, mixed)   # geometric middle of 36 / 32 and 160 / 32: 2.4
     pool.check()
     pool.release()
+
+
+def test_gates_of_any_size(cuda_device):
+    """One cell, whose weight is 1: v times the gate's sigmoid, from closed gates (denormal) to open ones."""
+    pool = KvPool(0, 1, 2, 128, 1, kv8="int8")
+    fill(pool, 3)
+    v = (pool.kv8_view(1, 0)[0].double() * pool.kv8_view(1, 0)[1].double()[..., None, None])[0, :, 0].repeat_interleave(4, 0)   # [8 heads][128]
+    gate = torch.linspace(-104, 104, 8 * 128, device="cuda").view(1, 8, 128)
+    gate[0, 0, 0], gate[0, 7, 127] = -INF, INF
+    q = torch.randn(1, 8, 128, device="cuda")
+    out = kv8_attend(pool, 0, q, dev([[0]]), dev([1]), 16, kv8_workspace(pool, 1, 8), gate=gate, gate_head_stride=128)[0].double()
+    want = v * torch.sigmoid(gate[0].double())
+    # two exponentials of base 2 and a division in front of the gate (2^-21 each at most, ex2.approx' bound), then expf (an ulp or two: 2^-22),
+    # a sum, a quotient and a product of half a step each; at the denormal end a step of 2^-149 in the sigmoid and one in the product
+    tol = want.abs() * (3 * 2.0 ** -21 + 2.0 ** -21) + (v.abs() + 1) * 2.0 ** -148
+    assert ((out - want).abs() <= tol).all(), ((out - want).abs() - tol).max()
+    pool.check()
+    pool.release()
