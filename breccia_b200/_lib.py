@@ -26,6 +26,7 @@ DTYPE_BF16 = 2
 
 KV8_CODES = {"e4m3": 1, "int8": 2}
 ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+ROPE_SIGNED = 256
 ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
 
 

@@ -201,8 +201,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // Read as a signed number it lies in [-1/2, 1/2) turns; times two that is sincospi's argument.  Sine, cosine and the factor
 // in 64 bits and one rounding to f32: a pair is computed once for all heads of a token, and a wrong last bit of it
 // shows as a neighbouring 8-bit code wherever a rotated key lies on a border.
-__device__ __forceinline__ float2 rope_cos_sin(uint32_t pos, uint64_t turns, double factor) {
-    const int64_t f = (int64_t)((uint64_t)pos * turns);
+// A negative position, as its 64-bit two's complement, turns backwards.
+__device__ __forceinline__ float2 rope_cos_sin(uint64_t pos, uint64_t turns, double factor) {
+    const int64_t f = (int64_t)(pos * turns);
     double s, c;
     sincospi((double)f * 0x1p-63, &s, &c);
     return make_float2((float)(c * factor), (float)(s * factor));

@@ -28,8 +28,12 @@ struct RopeParams {
     RopeSide side[2];
     const uint32_t *positions;
     const uint64_t *turns;
-    uint32_t n_tokens, tokens_per_cta, splits, head_dim, n_rot, interleaved;
+    uint32_t n_tokens, tokens_per_cta, splits, head_dim, n_rot, interleaved, is_signed;
     double factor;
+    __device__ __forceinline__ uint64_t position(uint32_t tok) const {
+        const uint32_t x = positions[tok];
+        return is_signed ? (uint64_t)(int64_t)(int32_t)x : x;
+    }
 };
 
 // Sixteen bytes of a row in f32.
@@ -98,7 +102,7 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32, 3) rope_kernel(const RopePara
         }
     };
     load(r);
-    const uint32_t pos = p.positions[tok];
+    const uint64_t pos = p.position(tok);
     for (uint32_t j = lane; j < half; j += 32u) pairs[j] = brc::rope_cos_sin(pos, p.turns[j], p.factor);
     __syncwarp();
     // cos and sin of the lane's columns (INTERLEAVED: of its pairs); the sine with the sign that a column's partner enters with
@@ -197,7 +201,7 @@ __global__ void __launch_bounds__(256) rope_any_kernel(const RopeParams p) {
     const uint32_t tok0 = blockIdx.x * p.tokens_per_cta;
     const uint32_t n_tok = min(p.tokens_per_cta, p.n_tokens - tok0), half = p.n_rot / 2u, hd = p.head_dim;
     for (uint32_t i = threadIdx.x; i < n_tok * half; i += blockDim.x)
-        cos_sin[i] = brc::rope_cos_sin(p.positions[tok0 + i / half], p.turns[i % half], p.factor);
+        cos_sin[i] = brc::rope_cos_sin(p.position(tok0 + i / half), p.turns[i % half], p.factor);
     __syncthreads();
     const uint32_t items = half + (hd - p.n_rot);   // pairs, then single untouched values
     for (uint32_t side = 0; side < 2; ++side) {
@@ -317,6 +321,8 @@ brc_status brc_rope_apply(int32_t device, const void *q_dev, void *q_out_dev, ui
     const char *who = "brc_rope_apply";
     if (dtype != BRC_DTYPE_F32 && dtype != BRC_DTYPE_F16 && dtype != BRC_DTYPE_BF16)
         return brc_fail(BRC_ERR_INVALID, "%s: dtype %d is none of f32 (0), f16 (1), bf16 (2)", who, dtype);
+    const bool is_signed = layout & BRC_ROPE_SIGNED;
+    layout &= ~BRC_ROPE_SIGNED;
     if (layout != BRC_ROPE_HALF && layout != BRC_ROPE_INTERLEAVED)
         return brc_fail(BRC_ERR_INVALID, "%s: layout %d is neither half (0) nor interleaved (1)", who, layout);
     if (head_dim == 0 || head_dim > 1024u) return brc_fail(BRC_ERR_UNSUPPORTED, "%s: head_dim %u (1 .. 1024)", who, head_dim);
@@ -374,6 +380,7 @@ brc_status brc_rope_apply(int32_t device, const void *q_dev, void *q_out_dev, ui
     p.head_dim = head_dim;
     p.n_rot = n_rot;
     p.interleaved = layout == BRC_ROPE_INTERLEAVED;
+    p.is_signed = is_signed;
     p.factor = factor;
     int sm_count = 0;
     BRC_CUDA(cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, device));

@@ -571,8 +571,9 @@ class Rope:
 
     def apply(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, q_out: torch.Tensor | None = None,
               k_out: torch.Tensor | None = None, stream=None):
-        """q [tokens, n_head, head_dim], k [tokens, n_kv, head_dim] or None, positions [tokens] int32 -> (q_out, k_out), new
-        tensors unless given (q_out=q rotates in place).  Tokens may be strided (columns of one projection)."""
+        """q [tokens, n_head, head_dim], k [tokens, n_kv, head_dim] or None, positions [tokens] int32 (a negative one turns
+        backwards) or uint32 -> (q_out, k_out), new tensors unless given (q_out=q rotates in place).  Tokens may be strided
+        (columns of one projection)."""
         tokens, hd, dtype = q.shape[0], q.shape[-1], q.dtype
         qo, qh, qs, qos = self._side("q", q, q_out, tokens, hd, dtype, stream)
         if k is None:
@@ -582,7 +583,8 @@ class Rope:
             k_ptr, ko_ptr = k.data_ptr(), ko.data_ptr()
         at = _words(positions, self.device, "Rope.apply: positions", tokens)
         _lib.check(self._call(self.device, q.data_ptr(), qo.data_ptr(), qh, qs, qos, k_ptr, ko_ptr, kh, ks, kos, hd,
-                              _dtype(dtype, "Rope.apply"), at, tokens, self._turns_ptr, self.n_rot, self.layout, self.factor,
+                              _dtype(dtype, "Rope.apply"), at, tokens, self._turns_ptr, self.n_rot,
+                              self.layout if positions.dtype == torch.uint32 else self.layout | _lib.ROPE_SIGNED, self.factor,
                               _raw_stream(stream, self.device)))
         return qo, ko
 

@@ -427,7 +427,10 @@ BRC_API brc_status brc_kv8_attn_ragged(brc_pool *pool, uint32_t layer, const voi
  * 64 bits); dims at and past n_rot are
  * copied.  Token strides in elements, 0: packed.  An output may be its input, the
  * same rows; otherwise the two must not overlap, and neither output may touch the
- * other side's rows (columns of one wider row are apart): refused. */
+ * other side's rows (columns of one wider row are apart): refused.
+ * layout: BRC_ROPE_HALF or _INTERLEAVED, with BRC_ROPE_SIGNED added where positions
+ * are int32_t: a negative one turns backwards (taken as uint32_t otherwise). */
+#define BRC_ROPE_SIGNED 256
 #define BRC_ROPE_NONE 0
 #define BRC_ROPE_LINEAR 1
 #define BRC_ROPE_NTK 2

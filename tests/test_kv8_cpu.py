@@ -143,3 +143,10 @@ def test_ragged_attention_refusals():
     assert call() == _lib.ERR_CUDA and b"brc_kv8_attn_ragged" in L.brc_last_error()
     assert call(cu=None) == _lib.ERR_INVALID and b"NULL prefix" in L.brc_last_error()
     assert call(pool=None) == _lib.ERR_INVALID
+
+
+def test_rope_layouts_with_signed_positions():
+    L, d = _lib.load(), 0x1000
+    for layout, ok in ((0, True), (1, True), (256, True), (257, True), (2, False), (258, False), (512, False), (-1, False)):
+        rc = L.brc_rope_apply(0, d, d, 1, 0, 0, None, None, 0, 0, 0, 64, 0, d, 0, d, 64, layout, 1.0, None)
+        assert (rc == 0) == ok and (ok or rc == _lib.ERR_INVALID), layout

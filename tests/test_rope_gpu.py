@@ -144,3 +144,22 @@ def test_refusals(cuda_device):
         with pytest.raises(BrcError):
             bad()
     assert rope.apply(x[:0], None, pos[:0])[0].shape == (0, 2, 128)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("hd,n_rot", [(128, 128), (256, 90), (80, 80)])   # rows of the wide kernel, of its odd pairing, of the other one
+def test_negative_positions_turn_backwards(cuda_device, layout, hd, n_rot):
+    rope = Rope(n_rot, theta=THETA, layout=layout, scaling="linear", factor=4.0)
+    x = torch.randn(6, 3, hd, device="cuda", generator=torch.Generator(device="cuda").manual_seed(7))
+    pos = np.array([-1, -7, -131072, -2 ** 31, 0, 9], np.int32)
+    xn, freqs = x.double().cpu().numpy(), ref.rope_freqs(n_rot, THETA, "linear", 4.0)
+    slack = 2.0 ** -51 * np.abs(pos[:, None, None].astype(np.float64)) * np.abs(xn).max() * 2   # as in test_scalings_layouts_types
+    y, _ = rope.apply(x, None, torch.from_numpy(pos).cuda())
+    want = ref.rotate(xn, pos, freqs, layout)
+    assert (np.abs(y.double().cpu().numpy() - want) <= tolerance(xn, want, 1.0, torch.float32) + slack).all()
+    # unsigned words are what they say: the same bits far forward
+    y, _ = rope.apply(x, None, torch.from_numpy(pos.view(np.uint32)).cuda())
+    far = pos.astype(np.int64) % 2 ** 32
+    want = ref.rotate(xn, far, freqs, layout)
+    slack = 2.0 ** -51 * far[:, None, None].astype(np.float64) * np.abs(xn).max() * 2
+    assert (np.abs(y.double().cpu().numpy() - want) <= tolerance(xn, want, 1.0, torch.float32) + slack).all()
