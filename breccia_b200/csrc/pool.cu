@@ -471,6 +471,10 @@ brc_status brc_pool_check(brc_pool *pool, void *stream) {
     if (w & BRC_DEV_WAIT_LIMIT)
         return brc_fail(BRC_ERR_TIMEOUT, "a kernel gave up a bounded wait (check word 0x%x, detail %u, at %u of %u)", w, detail,
                         pool->status_host[2], pool->status_host[3]);
+    if (w == BRC_DEV_BAD_VALUE)   // nothing was refused: the write took place
+        return brc_fail(BRC_ERR_DEVICE_CHECK,
+                        "an infinity or NaN reached a quantising write, which stored the largest code or 0 for it (check word 0x%x, source "
+                        "row %u or a later one of its page)", w, detail);
     return brc_fail(BRC_ERR_DEVICE_CHECK,
                     "a kernel refused an index: check word 0x%x (%s%s%s%s), last offending value %u", w,
                     (w & BRC_DEV_BAD_PAGE) ? "page id >= n_pages " : "", (w & BRC_DEV_BAD_POS) ? "position past bound " : "",

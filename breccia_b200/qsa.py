@@ -96,7 +96,7 @@ class KvPool:
         _lib.call("brc_pool_poison_nan", self.handle, _stream_ptr(stream))
 
     def check(self, stream=None) -> None:
-        """Synchronise and raise if any kernel refused an index or gave up a wait."""
+        """Synchronise and raise if any kernel refused an index, gave up a wait or met an infinity or NaN in a quantising write."""
         _lib.call("brc_pool_check", self.handle, _stream_ptr(stream))
 
     def k_ptr(self, layer: int) -> int:

@@ -50,7 +50,7 @@ typedef int32_t brc_status;
 #define BRC_ERR_CUDA (-3)         /* a CUDA runtime / driver call failed          */
 #define BRC_ERR_NO_PAGES (-4)     /* allocator has too few free pages             */
 #define BRC_ERR_TIMEOUT (-5)      /* a bounded device-side wait gave up           */
-#define BRC_ERR_DEVICE_CHECK (-6) /* a kernel's own bounds check refused an index */
+#define BRC_ERR_DEVICE_CHECK (-6) /* a kernel's own check refused an index or reports a value */
 #define BRC_ERR_UNSUPPORTED (-7)  /* geometry outside what the kernels are built for */
 #define BRC_ERR_NOT_RESIDENT (-8) /* page is in the host tier                     */
 
@@ -162,7 +162,8 @@ BRC_API brc_status brc_pool_write(brc_pool *pool, int32_t which, uint32_t layer,
                                   const void *src, uint64_t bytes, void *stream);
 /* Synchronises `stream`, then reports and clears the device-side check word:
  * BRC_OK, BRC_ERR_DEVICE_CHECK (an out-of-range page id or position reached a
- * kernel, which skipped the access) or BRC_ERR_TIMEOUT (a bounded wait gave
+ * kernel, which skipped the access; or an infinity or NaN reached a quantising
+ * write, which went on) or BRC_ERR_TIMEOUT (a bounded wait gave
  * up).  Mirrors the reference's bounded fence wait
  * (crates/breccia-vk/src/ctx.rs:1541-1561) without aborting the process. */
 BRC_API brc_status brc_pool_check(brc_pool *pool, void *stream);

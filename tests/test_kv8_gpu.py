@@ -856,3 +856,19 @@ def test_gates_of_any_size(cuda_device):
     assert ((out - want).abs() <= tol).all(), ((out - want).abs() - tol).max()
     pool.check()
     pool.release()
+
+
+def test_what_check_says_of_an_infinity(cuda_device):
+    """The write took place, so no index was refused; beside a refused one both are named."""
+    pool = KvPool(0, 1, 2, 128, 2, kv8="int8")
+    k = torch.ones(20, 2, 128, device="cuda")
+    k[17, 1, 3] = INF
+    kv8_append(pool, 0, k, k, dev([[0, 1]]), dev([0]), 20, tokens_per_seq=20)
+    with pytest.raises(BrcError, match="infinity or NaN reached a quantising write, which stored") as e:
+        pool.check()
+    assert "refused" not in str(e.value) and "row 16" in str(e.value)   # the first row of its page
+    kv8_append(pool, 0, k, k, dev([[7, 1]]), dev([0]), 20, tokens_per_seq=20)
+    with pytest.raises(BrcError, match="refused an index.*page id.*infinity or NaN"):
+        pool.check()
+    pool.check()
+    pool.release()
