@@ -9,6 +9,8 @@
 // their way.  Bound: HBM for chunks (source rows once, one byte per value written), the launch for a decode step.
 //
 // brc_kv8_read: the inverse, one CTA per (page, side); HBM.
+#include <algorithm>
+
 #include "brc_internal.h"
 #include "kv8.cuh"
 
@@ -390,11 +392,17 @@ brc_status brc_kv8_append(brc_pool *pool, uint32_t layer, const uint32_t *block_
     p.k_vec = ((reinterpret_cast<uintptr_t>(k_src_dev) | (k_token_stride * size)) & 15u) == 0;
     p.v_vec = ((reinterpret_cast<uintptr_t>(v_src_dev) | (v_token_stride * size)) & 15u) == 0;
     const uint64_t tiles = brc::tile_slots(total_tokens, n_seqs);
-    // All heads of a page in one CTA once that still leaves every SM several (the search, the positions' cos and sin and the
-    // start are then paid once, and the next head's rows travel while one is encoded), one head a CTA for a decode step.  16 000 tokens of
-    // 8 heads of 128 in bf16: 25.4 us with all eight, 27.4 with four, 29.8 with two, 37.8 with one.
-    p.heads_per_cta = tiles * 2u >= 4ull * pool->sm_count ? pool->n_kv_head : 1u;
-    const dim3 grid((uint32_t)tiles, 2u * ((pool->n_kv_head + p.heads_per_cta - 1u) / p.heads_per_cta));
+    // Heads a CTA: as many as leave an SM five CTAs with work (the search, the positions' cos and sin and the start are then paid
+    // once for several heads, and the next head's rows travel while one is encoded).  Pages that the call touches are counted from below; of
+    // the slots, a decode step leaves every other one idle.  One, two, four, eight heads a CTA, one token each in 8 heads of 128, bf16,
+    // rotated: 32 sequences 4.2, 5.0, 6.6, 9.8 us (one taken); 64: 6.2, 5.2, 6.9, 10.1 (two); 144: 10.1, 8.0, 8.1, 10.5 (four); 512: 27.8, 19.6,
+    // 15.9, 15.8 (eight); one sequence of 5000 tokens 16.7, 12.9, 11.9, 13.0 (four); 64 of 100 25.8, 19.3, 17.4, 17.4 (eight).
+    // Two heads of 256, where a CTA takes one up to 185 pages: 144 sequences 5.7 and 6.2 rotated, 4.3 and 3.7 not.
+    const uint64_t pages = std::max<uint64_t>(total_tokens / 16u, std::min(n_seqs, total_tokens)), want = 5ull * pool->sm_count;
+    const uint32_t most = (uint32_t)std::min<uint64_t>((2u * pages * pool->n_kv_head + want - 1u) / want, pool->n_kv_head);
+    const uint32_t groups = (pool->n_kv_head + most - 1u) / most;
+    p.heads_per_cta = (pool->n_kv_head + groups - 1u) / groups;
+    const dim3 grid((uint32_t)tiles, 2u * groups);
     brc_stage_begin(pool, BRC_STAGE_KV_APPEND, brc_stream(stream));
     const cudaError_t e = BRC_KV8_DISPATCH(launch_append, pool, src_dtype, p, pool->head_dim, grid, brc_stream(stream));
     brc_stage_end(pool, BRC_STAGE_KV_APPEND, brc_stream(stream));

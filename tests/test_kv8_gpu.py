@@ -872,3 +872,25 @@ def test_what_check_says_of_an_infinity(cuda_device):
         pool.check()
     pool.check()
     pool.release()
+
+
+@pytest.mark.parametrize("n_seqs,n_kv,hd,dtype,n", [(160, 5, 128, "bf16", 1), (70, 8, 128, "f16", 1), (150, 2, 256, "f32", 1), (1, 7, 128, "f16", 3000), (300, 3, 128, "bf16", 2)])
+def test_append_with_some_heads_a_cta(cuda_device, n_seqs, n_kv, hd, dtype, n):
+    """Calls whose heads are dealt out in groups, the last one smaller: every head once, kept cells in front of the new ones."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    first = np.random.default_rng(1).integers(1, 15, n_seqs)
+    tables, n_pages = scattered(3, first + n)
+    pool, cache = KvPool(0, 1, n_kv, hd, n_pages, kv8="e4m3"), ref.Cache(n_pages, n_kv, hd, "e4m3")
+    pool.poison_nan()
+    at, t = np.zeros(n_seqs, np.int64), dev(tables)
+    for counts in (first, np.full(n_seqs, n)):
+        cu = np.concatenate([[0], np.cumsum(counts)])
+        k, v = (random_rows(g, int(cu[-1]), n_kv, hd, dtype) for _ in range(2))
+        kv8_append(pool, 0, k, v, t, dev(at), int((at + counts).max()), cu_tokens=dev(cu))
+        kn, vn = k.double().cpu().numpy(), v.double().cpu().numpy()
+        for s in range(n_seqs):
+            cache.append(tables[s], int(at[s]), kn[cu[s]:cu[s + 1]], vn[cu[s]:cu[s + 1]])
+        at += counts
+    pool.check()
+    assert_pool_is(pool, cache, tables, at)
+    pool.release()
