@@ -646,9 +646,10 @@ def kv8_attend(pool: KvPool, layer: int, q: torch.Tensor, block_tables: torch.Te
                out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None, gate: torch.Tensor | None = None,
                gate_head_stride: int = 0, stream=None) -> torch.Tensor:
     """Attention over an 8-bit pool for the last T tokens of each sequence (brc_kv8_attn): q [tokens, n_head, hd], T = max_q, or
-    ragged by cu_q [n_seqs + 1] int32 with T <= max_q (rows past q's end are left out and reported by check()); token i of T sees seq_lens[s] - (T - 1 - i) cells.  Sums and softmax
-    in f32, probabilities to 22 bits, one rounding to `out_dtype` (q's type unless given).  `out` may be q.
-    `workspace` from kv8_workspace; calls that may run at the same time need one each."""
+    ragged by cu_q [n_seqs + 1] int32 with T <= max_q (rows past q's end are left out and reported by check(); rows that are no
+    sequence's are left as they were); token i of T sees seq_lens[s] - (T - 1 - i) cells.  Sums and softmax in f32, probabilities
+    to 22 bits, one rounding to `out_dtype` (q's type unless given).  `out` may be q.  `workspace` from kv8_workspace; calls that
+    may run at the same time need one each."""
     device = pool.device
     n_seqs, stride = block_tables.shape
     if q.dim() != 3 or q.shape[2] != pool.head_dim or not q.is_contiguous() or q.get_device() != device:
@@ -667,13 +668,13 @@ def kv8_attend(pool: KvPool, layer: int, q: torch.Tensor, block_tables: torch.Te
     elif out.data_ptr() < q.data_ptr() + q.nbytes and q.data_ptr() < out.data_ptr() + out.nbytes and \
             not (out.data_ptr() == q.data_ptr() and out.dtype == q.dtype):
         raise BrcError(_lib.ERR_INVALID, "kv8_attend: out overlaps q without being the same rows")
-    if gate is not None and gate.numel() and tokens:
-        has = 1 + sum((n - 1) * s for n, s in zip(gate.shape, gate.stride()))
-        if has < (tokens * n_head - 1) * gate_head_stride + hd:
+    if gate is not None and tokens:
+        has = 1 + sum((n - 1) * s for n, s in zip(gate.shape, gate.stride())) if gate.numel() else 0
+        if gate_head_stride < hd or has < (tokens * n_head - 1) * gate_head_stride + hd:
             raise BrcError(_lib.ERR_INVALID, f"kv8_attend: gate {tuple(gate.shape)} with strides {gate.stride()} for {tokens * n_head} rows of {hd} every {gate_head_stride} values")
-    if workspace.get_device() != device or (gate is not None and (gate.get_device() != device or gate.dtype != torch.float32)):
-        raise BrcError(_lib.ERR_INVALID, f"kv8_attend: workspace on {workspace.device}, gate {None if gate is None else (gate.dtype, gate.device)}: "
-                                         f"cuda:{device} and float32 wanted")
+    if workspace.get_device() != device or not workspace.is_contiguous() or (gate is not None and (gate.get_device() != device or gate.dtype != torch.float32)):
+        raise BrcError(_lib.ERR_INVALID, f"kv8_attend: workspace {tuple(workspace.shape)} with strides {workspace.stride()} on {workspace.device}, gate {None if gate is None else (gate.dtype, gate.device)}: "
+                                         f"contiguous on cuda:{device}, and a gate in float32, wanted")
     L, rows = _lib.load(), () if cu is None else (tokens,)
     _lib.check((L.brc_kv8_attn if cu is None else L.brc_kv8_attn_ragged)(
         pool.handle, layer, q.data_ptr(), _dtype(q.dtype, "kv8_attend"), *rows, n_head, None if gate is None else gate.data_ptr(), gate_head_stride,

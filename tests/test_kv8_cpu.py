@@ -150,3 +150,19 @@ def test_rope_layouts_with_signed_positions():
     for layout, ok in ((0, True), (1, True), (256, True), (257, True), (2, False), (258, False), (512, False), (-1, False)):
         rc = L.brc_rope_apply(0, d, d, 1, 0, 0, None, None, 0, 0, 0, 64, 0, d, 0, d, 64, layout, 1.0, None)
         assert (rc == 0) == ok and (ok or rc == _lib.ERR_INVALID), layout
+
+
+def test_attention_arguments_that_describe_no_memory():
+    """Strides and views that the library, given an address and a size, would read past: refused in front of it (which would answer
+    ERR_CUDA for this pool without a device)."""
+    from breccia_b200.qsa import KvPool, kv8_attend
+
+    pool = KvPool(0, 1, 2, 128, 8, bookkeeping_only=True)
+    pool.device = -1   # where CPU tensors lie
+    q, t, n, ws = torch.ones(2, 4, 128), torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32), torch.zeros(1 << 20, dtype=torch.uint8)
+    gate = torch.ones(2, 4, 128)
+    for bad in (dict(gate=gate, gate_head_stride=-128), dict(gate=gate, gate_head_stride=0), dict(gate=gate, gate_head_stride=64),
+                dict(gate=gate[:1], gate_head_stride=128), dict(gate=gate[:0], gate_head_stride=128), dict(ws=ws[:1].expand(1 << 20)), dict(ws=ws[::2])):
+        with pytest.raises(_lib.BrcError) as e:
+            kv8_attend(pool, 0, q, t, n, 16, bad.pop("ws", ws), **bad)
+        assert e.value.code == _lib.ERR_INVALID, bad
