@@ -253,7 +253,8 @@ void launch(RopeParams &p, bool rows, uint32_t total_heads, int sm_count, cudaSt
     p.tokens_per_cta = std::min(std::max(1u, 32768u / bytes), std::max(1u, 8192u / p.n_rot));
     p.tokens_per_cta = std::min(p.tokens_per_cta, std::max(1u, p.n_tokens / 296u));
     const uint32_t smem = p.tokens_per_cta * (p.n_rot / 2u) * (uint32_t)sizeof(float2);
-    rope_any_kernel<DT><<<(p.n_tokens + p.tokens_per_cta - 1u) / p.tokens_per_cta, 256, smem, st>>>(p);
+    const uint32_t grid = (uint32_t)(((uint64_t)p.n_tokens + p.tokens_per_cta - 1u) / p.tokens_per_cta);
+    rope_any_kernel<DT><<<grid, 256, smem, st>>>(p);
 }
 
 struct Rows {   // n of them: `bytes` each, from `at`, `stride` bytes apart

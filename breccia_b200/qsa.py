@@ -575,6 +575,8 @@ class Rope:
         backwards) or uint32 -> (q_out, k_out), new tensors unless given (q_out=q rotates in place).  Tokens may be strided
         (columns of one projection)."""
         tokens, hd, dtype = q.shape[0], q.shape[-1], q.dtype
+        if tokens >= 1 << 32:
+            raise BrcError(_lib.ERR_UNSUPPORTED, f"Rope.apply: {tokens} tokens in one call (below 2^32)")
         qo, qh, qs, qos = self._side("q", q, q_out, tokens, hd, dtype, stream)
         if k is None:
             ko, k_ptr, ko_ptr, kh, ks, kos = None, None, None, 0, 0, 0

@@ -166,3 +166,15 @@ def test_attention_arguments_that_describe_no_memory():
         with pytest.raises(_lib.BrcError) as e:
             kv8_attend(pool, 0, q, t, n, 16, bad.pop("ws", ws), **bad)
         assert e.value.code == _lib.ERR_INVALID, bad
+
+
+def test_rope_refuses_more_tokens_than_a_call_counts():
+    """2^32 + 1 rows are one row to a 32-bit count; meta tensors have the shape without the memory."""
+    from breccia_b200.qsa import Rope
+
+    rope = Rope(2)
+    rope.device = -1   # where meta tensors lie
+    for n in (2 ** 32, 2 ** 32 + 1):
+        x, pos = torch.empty(n, 1, 2, dtype=torch.float16, device="meta"), torch.empty(n, dtype=torch.int32, device="meta")
+        with pytest.raises(_lib.BrcError, match="tokens"):
+            rope.apply(x, None, pos, q_out=x)
