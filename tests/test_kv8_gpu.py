@@ -894,3 +894,91 @@ def test_append_with_some_heads_a_cta(cuda_device, n_seqs, n_kv, hd, dtype, n):
     pool.check()
     assert_pool_is(pool, cache, tables, at)
     pool.release()
+
+
+def rotation_error(x, m=1.0):
+    """test_rope_gpu.tolerance: f32 arithmetic on a pair, 8 * 2^-24 * 2 max|x| m."""
+    return 8 * 2.0 ** -24 * 2 * np.abs(x).max() * m
+
+
+def code_steps(x, scale, code):
+    """Distance between neighbouring codes around x, in x's units."""
+    return ref.step_of(x / scale, code) * scale
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("layout,n_rot,offset", [("half", 256, 0), ("half", 64, 0), ("half", 90, 0), ("half", 128, 1), ("interleaved", 256, 0), ("interleaved", 90, 1)])
+def test_append_rotates_keys_of_256(cuda_device, code, dtype, layout, n_rot, offset):
+    """Heads of 256, whose rows are half a block: every pairing, aligned and not, one token and chunks; V as it comes."""
+    n_kv, hd = 2, 256
+    counts, pos0 = [40, 1, 19], [70003, 16, 5]
+    own, n_pages = scattered(5, [p % 16 + n for p, n in zip(pos0, counts)])
+    wide = np.zeros((3, max(pos0) // 16 + own.shape[1]), np.int32)
+    for s, p in enumerate(pos0):
+        wide[s, p // 16:p // 16 + own.shape[1]] = own[s]
+    g = torch.Generator(device="cuda").manual_seed(2)
+    total, row = sum(counts), 2 * n_kv * hd + offset
+    m = torch.randn(total * row + offset, device="cuda", generator=g).to(DTYPES[dtype])[offset:].view(total, row)
+    pool = KvPool(0, 1, n_kv, hd, n_pages, kv8=code)
+    rope = Rope(n_rot, theta=500000.0, layout=layout, scaling="yarn", factor=16.0, orig_ctx=8192)
+    cu, end = np.concatenate([[0], np.cumsum(counts)]), max(p + n for p, n in zip(pos0, counts))
+    kv8_append(pool, 0, m[:, :n_kv * hd], m[:, n_kv * hd:2 * n_kv * hd], dev(wide), dev(pos0), end, cu_tokens=dev(cu), rope=rope)
+    got = [x.double().cpu().numpy() for x in kv8_read(pool, 0, dev(wide), dev(pos0), end, cu_tokens=dev(cu), total_tokens=total, dtype=torch.float32)]
+    pool.check()
+    pos = np.concatenate([np.arange(p, p + n) for p, n in zip(pos0, counts)])
+    rows = m.double().cpu().numpy()
+    xk = ref.rotate(rows[:, :n_kv * hd].reshape(total, n_kv, hd), pos, ref.rope_freqs(n_rot, 500000.0, "yarn", 16.0, 8192), layout, rope.factor)
+    xv = rows[:, n_kv * hd:2 * n_kv * hd].reshape(total, n_kv, hd)
+    page = np.array([wide[np.searchsorted(cu, a, "right") - 1, pos[a] // 16] for a in range(total)])
+    for side, (x, fuzz) in enumerate(((xk, rotation_error(rows, rope.factor)), (xv, 0.0))):
+        scale = pool.kv8_view(side, 0)[1].double().cpu().numpy()[page][:, :, None]
+        # half a step; K's f32 error moves a value, and with it the border that it is rounded at
+        assert (np.abs(got[side] - x) <= code_steps(x, scale, code) / 2 + 2 * fuzz).all(), np.abs(got[side] - x).max()
+        for i in np.unique(page):   # and no scale larger than the page needs
+            amax = np.abs(x[page == i]).max((0, 2))
+            assert all(scale[page == i][0, h, 0] <= 2.0 ** ref.exponent(amax[h] + fuzz, code) for h in range(n_kv))
+    pool.release()
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_a_serving_run_stores_what_was_put_in(cuda_device, code, layout):
+    """Prompt, decode steps, drafts with a roll-back: after each of them every cached key and value lies within the code's rounding of the
+    exact one, and keys that were not rotated, or rotated the other way about, would not."""
+    n_kv, hd = 2, 128
+    tables, n_pages = scattered(1, [200, 200])
+    pool, t = KvPool(0, 1, n_kv, hd, n_pages, kv8=code), dev(tables)
+    rope = Rope(64, theta=500000.0, layout=layout, scaling="bands", factor=8.0, orig_ctx=8192)
+    freqs, g = ref.rope_freqs(64, 500000.0, "bands", 8.0, 8192), torch.Generator(device="cuda").manual_seed(6)
+    lens = np.array([0, 0])
+    none = np.zeros((0, n_kv, hd))
+    exact = [[none, none, none, none] for _ in range(2)]                        # keys, values; keys as they came, keys by the other layout
+    written = [[np.zeros((0, n_kv, 1))] * 2 for _ in range(2)]                  # each cell's scale when it was written
+    for counts, keep in (([90, 31], [90, 31]), ([1, 1], [1, 1]), ([4, 3], [2, 1]), ([1, 4], [1, 4]), ([20, 1], [20, 1]), ([1, 1], [1, 1])):
+        cu = np.concatenate([[0], np.cumsum(counts)])
+        k, v = (random_rows(g, int(cu[-1]), n_kv, hd, "f32") for _ in range(2))
+        pos = np.concatenate([np.arange(p, p + n) for p, n in zip(lens, counts)])
+        kv8_append(pool, 0, k, v, t, dev(lens), int((lens + counts).max()), cu_tokens=dev(cu), rope=rope)
+        pool.check()
+        raw = k.double().cpu().numpy()
+        new = [ref.rotate(raw, pos, freqs, layout), v.double().cpu().numpy(), raw, ref.rotate(raw, pos, freqs, "half" if layout == "interleaved" else "interleaved")]
+        fuzz = rotation_error(raw)
+        for s in range(2):
+            n = int(lens[s]) + counts[s]
+            now = [np.concatenate([a, b[cu[s]:cu[s + 1]]]) for a, b in zip(exact[s], new)]
+            held = [x.double().cpu().numpy() for x in kv8_read(pool, 0, dev(tables[s:s + 1]), dev([0]), n, tokens_per_seq=n, dtype=torch.float32)]
+            for side in (0, 1):
+                scale = pool.kv8_view(side, 0)[1].double().cpu().numpy()[tables[s][np.arange(n) // 16]][:, :, None]
+                written[s][side] = np.concatenate([written[s][side], scale[int(lens[s]):]])
+                # half a step of the present scale; a cell whose page has grown since was rounded at every smaller scale too: half a step of
+                # each, together at most another half of the present one
+                room = code_steps(now[side], scale, code) * np.where(scale > written[s][side], 1.0, 0.5) + (2 * fuzz if side == 0 else 0.0)
+                assert (np.abs(held[side] - now[side]) <= room).all(), (side, s, counts)
+                if side == 0 and n > 40:
+                    for wrong in now[2:]:
+                        assert (np.abs(held[0] - wrong) > code_steps(wrong, scale, code) + 2 * fuzz).mean() > 0.05
+            exact[s] = [x[: int(lens[s]) + keep[s]] for x in now]
+            written[s] = [x[: int(lens[s]) + keep[s]] for x in written[s]]
+        lens = lens + keep
+    pool.release()

@@ -163,3 +163,19 @@ def test_negative_positions_turn_backwards(cuda_device, layout, hd, n_rot):
     want = ref.rotate(xn, far, freqs, layout)
     slack = 2.0 ** -51 * far[:, None, None].astype(np.float64) * np.abs(xn).max() * 2
     assert (np.abs(y.double().cpu().numpy() - want) <= tolerance(xn, want, 1.0, torch.float32) + slack).all()
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("hd,n_rot", [(256, 256), (256, 192), (256, 90), (256, 8), (64, 64), (64, 24), (128, 100)])
+def test_every_row_kernel(cuda_device, layout, dtype, hd, n_rot):
+    """Rows of one and of two chunks a lane, pairs by shuffle within a chunk, across chunks and through shared memory, beside untouched values."""
+    rope = Rope(n_rot, layout=layout)
+    g = torch.Generator(device="cuda").manual_seed(hd + n_rot)
+    q, k = (torch.randn(37, h, hd, device="cuda", generator=g).to(DTYPES[dtype]) for h in (9, 2))
+    pos = np.arange(37, dtype=np.int32) * 977
+    out = rope.apply(q, k, torch.from_numpy(pos).cuda())
+    for x, y in zip((q, k), out):
+        xn = x.double().cpu().numpy()
+        check(y, xn, ref.rotate(xn, pos, ref.rope_freqs(n_rot, 10000.0), layout), 1.0, DTYPES[dtype])
+        assert torch.equal(y[..., n_rot:], x[..., n_rot:])
