@@ -3,7 +3,7 @@
 //
 //   out[i,h] = sigmoid(gate) * sum_c softmax_c(scale * q.k_c) v_c,   c < len - (T - 1 - i)
 //
-// What bounds it: one token of 8 heads per kv head does 32 FLOP per cached byte, far under the 260 a B200's tensor cores
+// What bounds it: one token of 8 heads per kv head does 16 FLOP per cached byte, far under the 260 a B200's tensor cores
 // have per byte of HBM, so the cache stream is the floor - if converting it keeps up: 24 bytes per SM and clock have to
 // become binary16 operands.  Hence:
 //   - the codes go to the tensor cores as the exact binary16 numbers they are (cvt of e4m3 pairs; byte permute and one
@@ -12,7 +12,8 @@
 //   - mma.sync m16n8k16 with the CACHE as the 16-row operand and the query rows as the 8-column one.  tcgen05 would pad 8
 //     rows to 64 or 128 and want the converted operand written back to shared memory, twice the bytes the codes
 //     themselves cost; the warp-level form takes it from the registers the conversion leaves it in.  Its rate is
-//     not the limit: 32 of them per page and head against 350 clocks of HBM time;
+//     not the limit: 48 of them per page and head of 256 (16 for the scores, 32 for the weights' two parts) against 350
+//     clocks of HBM time; the pipe is busy 21 to 29 % of the time;
 //   - fragments are cut so that a thread's sixteen consecutive bytes are one 16-byte shared-memory read: the sum over
 //     head_dim may run in any order, so K's columns are dealt out 16 bytes to a thread, and V's columns likewise become
 //     the output rows; the 128-byte swizzle of the TMA box keeps every such read free of bank conflicts;
@@ -955,7 +956,9 @@ brc_status launch(const brc_pool *pool, AttnParams p, uint32_t grid, uint32_t me
     BRC_CUDA(cudaLaunchKernelEx(&cfg, kern, pool->tm_kv8, p));
     cfg.dynamicSmemBytes = 0;
     if ((uint64_t)p.n_seqs * p.units_per_seq * 8u <= grid) {
-        // Few units have many partials each (one long sequence: one from every SM): 16 warps a row fetch eighty at a time.
+        // Few units have many partials each (one long sequence: one from every SM): 16 warps a row fetch eighty at a time.  Whole call (us)
+        // with 16 warps a row and with one, 16 heads over 2 of 256 (a unit a sequence): 1 of 131 072 cells 32.9, 58.0; 8 of 4000-9000
+        // 21.0, 24.4; 12 25.7, 26.2; 18 33.3, 32.7; 32 of 512-8192 38.2, 33.6.  8 kv heads of 128 (four units): 4 sequences 20.7, 20.7; 24 77.9, 52.5.
         cfg.gridDim = dim3(p.n_seqs * p.units_per_seq, merge_rows);
         cfg.blockDim = dim3(512);
         BRC_CUDA(cudaLaunchKernelEx(&cfg, kv8_merge_kernel<HD, 16, 1, 5, RG == 2>, p, grid));
@@ -970,8 +973,8 @@ brc_status launch(const brc_pool *pool, AttnParams p, uint32_t grid, uint32_t me
 template <int HD, uint32_t CODE, bool SPLIT_Q, int KVB>
 brc_status launch_rows(const brc_pool *pool, const AttnParams &p, uint32_t grid, uint32_t rt, uint32_t merge_rows, cudaStream_t st) {
     // Warps: what the registers of the sums allow and the ring bears (a stage for each warp that takes pages in turn, twice
-    // over).  Measured (us) at 8, 12, 16 warps of head_dim 128: 32 sequences, 8 kv heads 54.4, 51.4, 53.5; drafts of 24 sequences 50.4, 50.2,
-    // 52.4; eight tokens each 79, 73, 84.
+    // over).  Measured (us) at 8 and 12 warps of head_dim 128: 32 sequences of 512-8192 cells, 8 kv heads 55.6, 50.4; drafts of 24
+    // sequences 53.4, 52.5; eight tokens each 87.3, 81.8; 7 heads over 7 58.6, 60.1.
     constexpr int W = HD == 128 ? 12 : 8;
     if (rt == 1) return launch<HD, CODE, SPLIT_Q, 1, 1, KVB, W>(pool, p, grid, merge_rows, st);
     return p.row_groups == 1 ? launch<HD, CODE, SPLIT_Q, 2, 1, KVB, W>(pool, p, grid, merge_rows, st) : launch<HD, CODE, SPLIT_Q, 2, 2, KVB, W>(pool, p, grid, merge_rows, st);
@@ -1059,9 +1062,10 @@ brc_status brc_kv8_attend(brc_pool *pool, const char *who, const brc_kv8_attn_ar
     p.units_per_seq = s.units_per_seq;
     p.scale_log2 = a.scale * 1.4426950408889634f;
     // Starting and finishing a unit takes a CTA about as long as streaming 128 KiB for each of the unit's heads, half as much again where
-    // two row tiles of 256 columns are merged.  Measured (us): 32 sequences of 512-8192 cells, 16 heads over 2 of 256: 33.2 at half of it,
-    // 32.8, 32.9 at one and a half times; with four tokens each 70.8, 66.1, 61.8, 62.1 at 128, 256, 384, 512 KiB; 7 heads over 7 of 128: 58.5 at 128 KiB,
-    // 62.4 at 256.
+    // two row tiles of 256 columns are merged.  Measured (us) at 64, 96, 128, 192, 256 KiB a head, sequences of 512-8192 cells, one row tile: 32 of
+    // 16 heads over 2 of 256 33.8, 33.1, 33.0, 33.4, 33.6; 32 heads over 8 of 128 50.6, 50.5, 50.5, 52.6, 54.3; 7 over 7 of 128 58.8, 59.2, 60.3, 63.1, 64.2.
+    // Two tiles of 128: drafts of 24 53.8, 51.6, 52.5, 55.1, 58.3.  Two tiles of 256: 16 heads over 2, two tokens 48.6, 47.2, 45.6, 43.3, 42.4, four
+    // 78.3, 75.8, 72.7, 68.8, 70.8; 8 over 1, four tokens 48.5, 47.4, 45.6, 43.5, 42.0.
     const uint32_t unit_kib = 128u * s.kvb * (s.rt == 2u && pool->head_dim == 256 ? 3u : 2u) / 2u;
     p.unit_cost = std::max(1u, unit_kib * 1024u / (s.kvb * 2u * 16u * pool->head_dim));
     const uint64_t most = (uint64_t)a.n_seqs * s.units_per_seq * ((a.max_seq_len + 15ull) / 16u + p.unit_cost);   // cost at most

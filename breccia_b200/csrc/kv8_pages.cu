@@ -92,8 +92,9 @@ __device__ __forceinline__ void rotate8(const PagesParams &p, const typename brc
 }
 
 // CTAs an SM that the compiler has to leave registers for: more of them hide the loads and barriers of one another until the
-// registers spill.  16 000 tokens, rotated, measured: 8 heads of 128, bf16, 34.1 us at 8, 35.4 at 7; 2 heads of 256, f16 22.7 at 5,
-// 24.6 at 4, f32 28.2 at 4, 31.6 at 3 (at 5, before sine and cosine went to 64 bits, 36.9 against 29.7 at 4).
+// registers spill.  16 000 tokens, measured (us) with one CTA fewer, as chosen, with one more.  8 heads of 128, rotated: bf16 (8) 35.3, 34.0, 34.0,
+// f32 (6) 44.3, 40.1, 40.7; as they come (9): bf16 25.2, 25.0, 26.0, f32 31.4, 31.4, 32.3.  2 heads of 256, rotated: f16 (5) 24.5, 22.6, 23.5,
+// f32 (4) 31.5, 28.3, 33.5; as they come: f16 (6) 15.3, 14.2, 14.9, f32 (4) 18.8, 18.8, 18.6.
 constexpr int append_ctas(int dt, int hd, bool rope) { return hd == 128 ? (rope ? (dt == 0 ? 6 : 8) : 9) : dt == 0 ? 4 : rope ? 5 : 6; }
 
 template <uint32_t CODE, int DT, int HD, bool ROPE>
