@@ -279,8 +279,7 @@ __device__ __forceinline__ void stage_q(const AttnParams &p, const Smem &L, uint
 }
 
 // RT: tiles of eight query rows that a warp carries; RG: warps side by side on a page's rows; KVB: kv heads of a unit; W: consuming
-// warps.  SPLIT_Q: q as two binary16 parts (f32 q; the 16-bit types are
-// exact in one).
+// warps.  SPLIT_Q: q as two binary16 parts (f32; of the 16-bit types one part loses only what lies under 2^-32 of the row's largest).
 template <int HD, uint32_t CODE, bool SPLIT_Q, int RT, int RG, int KVB, int W>
 __global__ void __launch_bounds__(W * 32 + 128, 1) kv8_attn_kernel(const __grid_constant__ CUtensorMap tm, const AttnParams p) {
     constexpr uint32_t SLABS = HD / 128, CONSUMERS = W * 32, ROW = HD + 4;
